@@ -1,0 +1,445 @@
+"""The operators of a served key-value cache that the framework is timed on.
+
+A cache holds every sequence's keys and values, either in the model's type or in 8 bits: e4m3 codes
+with one power-of-two scale (an exponent byte) for each token and KV head. It is a pool of blocks
+with block tables, or one slab per sequence. Four operators work on it:
+
+    "write"   new tokens' rows go into the cache, quantised where it holds 8 bits, and the rows are
+              read back as the values that attention will see
+    "read"    whole sequences come out of the cache as contiguous rows
+    "attend"  the new tokens of every sequence attend to their sequence's cache, causally (a chunk of
+              a prompt, a conversation's next turn, a few drafted tokens, a batch of all of these)
+    "cross"   a decoder's tokens attend to the states of an encoder, padded to the longest, unmasked
+    "decode"  one token per sequence attends to a cache in 8 bits
+
+Unwritten rows of a cache hold NaN, as memory that nobody has cleared may.
+
+    layout    "paged16", "paged64": a shuffled pool of blocks of 16 or 64 rows; "bshd": [B, S, H_kv, D]
+    tokens    new tokens of each sequence: all `new` ("equal"), or from one to `new`, spread over the
+              logarithm, with one sequence idle ("mixed")
+    lengths   of the sequences with the new tokens: all `longest`, or spread evenly from 1/B of it
+"""
+
+import math
+
+import torch
+
+own = False
+
+DTYPES = {"bf16": torch.bfloat16, "fp16": torch.float16}
+PAGES = {"paged16": 16, "paged64": 64, "bshd": 0}
+
+
+def _case(name, op, batch, heads, heads_kv, head_dim, dtype, cache, layout, new, tokens, longest,
+          capacity, lengths):
+    return dict(name=name, op=op, batch=batch, heads=heads, heads_kv=heads_kv, head_dim=head_dim,
+                dtype=dtype, cache=cache, layout=layout, new=new, tokens=tokens, longest=longest,
+                capacity=capacity, lengths=lengths)
+
+
+def listed():
+    return [
+        # A long prompt's keys and values go into an 8-bit pool.
+        _case("write_prompt_8k", "write", 1, 32, 8, 128, "bf16", "e4m3", "paged16", 8192, "equal",
+              8192, 8448, "equal"),
+        # One decode step of a serving batch: a row per sequence, where latency counts.
+        _case("write_step_24", "write", 24, 32, 8, 128, "bf16", "e4m3", "paged16", 1, "equal", 8000,
+              8192, "spread"),
+        # A shared prefix is taken out of the pool, to go on with in another layout.
+        _case("read_prefix_32k", "read", 1, 32, 8, 128, "bf16", "e4m3", "paged16", 0, "equal", 32768,
+              32768, "equal"),
+        # A small model's batch moves out of a pool in its own type, to another device or the host.
+        _case("read_batch_d64", "read", 16, 16, 16, 64, "fp16", "same", "paged64", 0, "equal", 1500,
+              1536, "spread"),
+        # A chunk of a long prompt whose earlier chunks lie in the 8-bit pool.
+        _case("attend_chunk_2048", "attend", 1, 32, 8, 128, "bf16", "e4m3", "paged16", 2048, "equal",
+              16384, 16384, "equal"),
+        # The next turn of a conversation, a few hundred tokens, on a pool in the model's type.
+        _case("attend_turn_300", "attend", 1, 32, 8, 128, "bf16", "same", "paged16", 300, "equal",
+              8492, 8512, "equal"),
+        # A serving batch in flight: sequences with one token, with a few, with a chunk of a prompt.
+        _case("attend_mixed_24", "attend", 24, 32, 8, 128, "bf16", "e4m3", "paged16", 512, "mixed",
+              8000, 8192, "spread"),
+        # Drafted tokens of several sequences are checked in one pass.
+        _case("attend_draft_5", "attend", 16, 64, 8, 128, "fp16", "e4m3", "paged64", 5, "equal", 4001,
+              4096, "spread"),
+        # A decoder's layer over the states of an encoder, of another length for every sequence.
+        _case("cross_8x200_d64", "cross", 8, 16, 16, 64, "fp16", "same", "bshd", 200, "equal", 2000,
+              2000, "spread"),
+        # The decode benchmark's batch on an 8-bit cache.
+        _case("decode_8x32k", "decode", 8, 32, 8, 128, "bf16", "e4m3", "bshd", 1, "equal", 32768,
+              32768, "equal"),
+        # A serving batch: conversations of different ages over an 8-bit pool.
+        _case("decode_paged_24", "decode", 24, 32, 8, 128, "bf16", "e4m3", "paged16", 1, "equal", 8000,
+              8192, "spread"),
+        # One interactive request after its short prompt, where latency counts.
+        _case("decode_short", "decode", 1, 32, 8, 128, "bf16", "e4m3", "paged16", 1, "equal", 640, 768,
+              "equal"),
+    ]
+
+
+# No drawn case has more products, cache bytes or (in the plain form) scores than the listed ones.
+MAX_FLOPS = 2.5e11
+MAX_CACHE_BYTES = 2.0**28
+MAX_SCORES = 2.0**30
+# (query heads, KV heads) of this repository's configurations, benchmarks and tests.
+HEADS = [(32, 32), (16, 16), (8, 8), (32, 8), (64, 8), (32, 4), (16, 2)]
+
+
+def _log_int(rng, low, high):
+    return int(round(math.exp(rng.uniform(math.log(low), math.log(high)))))
+
+
+def draw(rng):
+    op = rng.choice(["write", "read", "attend", "attend", "cross", "decode", "decode"])
+    heads, heads_kv = rng.choice(HEADS)
+    head_dim = rng.choice([128, 128, 64])
+    batch = _log_int(rng, 1, 32)
+    dtype = rng.choice(["bf16", "bf16", "fp16"])
+    cache = "e4m3" if op == "decode" else rng.choice(["e4m3", "same"])
+    layout = rng.choice(["paged16", "paged64", "bshd"])
+    lengths = rng.choice(["equal", "spread"])
+    tokens = "equal"
+    longest = _log_int(rng, 64, 32768)
+    new = 1
+    if op == "write":
+        new = min(longest, _log_int(rng, 1, 8192))
+        tokens = rng.choice(["equal", "mixed"])
+    elif op == "attend":
+        new = min(longest, _log_int(rng, 1, 2048))
+        tokens = rng.choice(["equal", "mixed"])
+    elif op == "cross":
+        new = _log_int(rng, 1, 512)
+        longest = min(longest, 4096)
+        layout = "bshd"
+    elif op == "read":
+        new = 0
+    elem = 1 if cache == "e4m3" else 2
+    while (2.0 * batch * heads_kv * longest * head_dim * elem > MAX_CACHE_BYTES
+           or batch * heads * max(new, 1) * float(longest) * (op not in ("write", "read")) > MAX_SCORES
+           or 4.0 * batch * heads * new * float(longest) * head_dim > MAX_FLOPS):
+        if batch > 1:
+            batch = (batch + 1) // 2
+        elif new > 512:
+            new -= new // 3
+        else:
+            longest -= longest // 3
+            new = min(new, longest)
+    # The cache is allocated for more tokens than it holds yet.
+    page = PAGES[layout] or 1
+    capacity = -(-(longest + rng.randint(0, longest // 4)) // page) * page
+    return {k: v for k, v in _case("", op, batch, heads, heads_kv, head_dim, dtype, cache, layout, new,
+                                   tokens, longest, capacity, lengths).items() if k != "name"}
+
+
+def _spread(n, seed):
+    """A fixed order of range(n)."""
+    return torch.randperm(n, generator=torch.Generator().manual_seed(seed)).tolist()
+
+
+def _sizes(case):
+    """The sequences' lengths and how many of their tokens are new (or read)."""
+    batch, longest, new = case["batch"], case["longest"], case["new"]
+    lens = [longest] * batch
+    if case["lengths"] == "spread":
+        lens = [max(1, longest * (i + 1) // batch) for i in _spread(batch, 1)]
+    if case["op"] == "read":
+        return lens, lens
+    counts = [new] * batch
+    if case["tokens"] == "mixed" and batch > 1:
+        counts = [int(round(new ** (i / (batch - 1)))) if i else 0 for i in _spread(batch, 2)]
+    if case["op"] != "cross":
+        lens = [max(n, c) for n, c in zip(lens, counts)]
+    return lens, counts
+
+
+def _quantise(x):
+    """e4m3 codes and the scales' exponent bytes of the rows of a float32 tensor: the scale is the
+    least power of two that brings the row's largest magnitude to at most 448."""
+    mantissa, exponent = torch.frexp(x.abs().amax(dim=-1, keepdim=True))
+    exponent = torch.where(mantissa > 0.875, exponent - 8, exponent - 9)
+    exponent = torch.where(mantissa > 0, exponent, 0).clamp(-126, 120)
+    codes = (x * _power(127 - exponent)).to(torch.float8_e4m3fn)
+    return codes, (exponent + 127).to(torch.uint8).squeeze(-1)
+
+
+def _power(biased):
+    """2^(biased - 127) as float32, from its exponent bits."""
+    return (biased.to(torch.int32) << 23).view(torch.float32)
+
+
+def _values(codes, exponents):
+    return codes.to(torch.float32) * _power(exponents).unsqueeze(-1)
+
+
+def _rows(gen, shape, dtype, head_dim):
+    """Rows as a model's projections give them: channels of different sizes."""
+    factor = torch.exp(0.5 * torch.randn(head_dim, device="cuda", generator=gen)).to(dtype)
+    x = torch.randn(shape, device="cuda", dtype=dtype, generator=gen)
+    return x.mul_(factor)
+
+
+def prepare(case, seed):
+    gen = torch.Generator(device="cuda").manual_seed(seed)
+    dtype, op, layout = DTYPES[case["dtype"]], case["op"], case["layout"]
+    batch, heads, heads_kv, head_dim = (case[k] for k in ("batch", "heads", "heads_kv", "head_dim"))
+    lens, counts = _sizes(case)
+    page, capacity = PAGES[layout], case["capacity"]
+    capacity = max(capacity, max(lens))
+    if page:
+        blocks = -(-capacity // page)
+        outer = (batch * blocks, page)
+        tables = torch.randperm(batch * blocks, device="cuda", generator=gen)
+        tables = tables.to(torch.int32).reshape(batch, blocks)
+    else:
+        outer = (batch, capacity)
+        tables = None
+    seq_lens = torch.tensor(lens, device="cuda", dtype=torch.int32)
+    ends = torch.tensor([0] + counts).cumsum(0).to(torch.int32)
+    s = dict(op=op, dtype=dtype, seq_lens=seq_lens, tables=tables, cu_seqlens=ends.to("cuda"),
+             total=sum(counts), most=max(counts), longest=max(lens), k_scales=None, v_scales=None)
+
+    # Which of the cache's rows hold a token: all but the rest of each sequence, and, before a write,
+    # all but the new ones.
+    held = torch.arange(capacity if not page else blocks * page, device="cuda")[None, :]
+    old = seq_lens - torch.tensor(counts, device="cuda", dtype=torch.int32) if op == "write" else seq_lens
+    held = held < old[:, None]
+    if page:
+        at_pool = torch.empty((batch * blocks, page), device="cuda", dtype=torch.bool)
+        at_pool[tables.flatten().long()] = held.reshape(batch * blocks, page)
+        held = at_pool
+    for name in ("k", "v"):
+        x = _rows(gen, (*outer, heads_kv, head_dim), dtype, head_dim)
+        if case["cache"] == "e4m3":
+            codes = torch.empty(x.shape, device="cuda", dtype=torch.uint8)
+            scales = torch.empty(x.shape[:-1], device="cuda", dtype=torch.uint8)
+            for part, c, e in zip(x.split(64), codes.split(64), scales.split(64)):
+                q, exponent = _quantise(part.float())
+                c.copy_(q.view(torch.uint8))
+                e.copy_(exponent)
+            codes[~held] = 0x7F
+            scales[~held] = 0xFF
+            s[f"{name}_cache"] = codes.view(torch.float8_e4m3fn)
+            s[f"{name}_scales"] = scales.view(torch.float8_e8m0fnu)
+        else:
+            x[~held] = math.nan
+            s[f"{name}_cache"] = x
+    if op == "write":
+        for name in ("k", "v"):
+            s[name] = _rows(gen, (s["total"], heads_kv, head_dim), dtype, head_dim)
+    elif op == "cross":
+        s["q"] = torch.randn((batch, case["new"], heads, head_dim), device="cuda", dtype=dtype, generator=gen)
+    elif op == "decode":
+        s["q"] = torch.randn((batch, 1, heads, head_dim), device="cuda", dtype=dtype, generator=gen)
+    elif op == "attend":
+        s["q"] = torch.randn((s["total"], heads, head_dim), device="cuda", dtype=dtype, generator=gen)
+    return s
+
+
+def _own(s):
+    import sys
+    from pathlib import Path
+
+    package = str(Path.cwd() / "flash-attention-lab_amd")
+    if package not in sys.path:
+        sys.path.insert(0, package)
+    import flash_lab
+
+    cache = dict(block_tables=s["tables"], k_scales=s["k_scales"], v_scales=s["v_scales"])
+    if s["op"] == "write":
+        flash_lab.write_cache(s["k"], s["v"], s["k_cache"], s["v_cache"], s["seq_lens"],
+                              cu_seqlens=s["cu_seqlens"], **cache)
+    if s["op"] in ("write", "read"):
+        return flash_lab.read_cache(s["k_cache"], s["v_cache"], s["seq_lens"], s["cu_seqlens"], s["total"],
+                                    dtype=s["dtype"], **cache)
+    if s["op"] == "decode":
+        return flash_lab.decode(s["q"], s["k_cache"], s["v_cache"], s["seq_lens"], return_lse=True, **cache)
+    if s["op"] == "cross":
+        return flash_lab.attention_cached(s["q"], s["k_cache"], s["v_cache"], s["seq_lens"], causal=False,
+                                          return_lse=True, **cache)
+    return flash_lab.attention_cached(s["q"], s["k_cache"], s["v_cache"], s["seq_lens"],
+                                      cu_seqlens=s["cu_seqlens"], return_lse=True, **cache)
+
+
+def _places(s, sequence, position):
+    """Rows of the flattened cache that hold these positions of these sequences."""
+    if s["tables"] is None:
+        return sequence * s["k_cache"].shape[1] + position
+    page = s["k_cache"].shape[1]
+    last = s["tables"].shape[1] - 1
+    block = s["tables"][sequence, (position // page).clamp(max=last)].long()
+    return block * page + position % page
+
+
+def _new_rows(s):
+    """Sequence, index within its new tokens, and position of each of the new tokens."""
+    counts = (s["cu_seqlens"][1:] - s["cu_seqlens"][:-1]).long()
+    sequence = torch.repeat_interleave(counts, output_size=s["total"])
+    index = torch.arange(s["total"], device="cuda") - s["cu_seqlens"].long()[sequence]
+    return sequence, index, s["seq_lens"].long()[sequence] - counts[sequence] + index
+
+
+def _plain_write(s, rows, name):
+    x, cache = s[name], s[f"{name}_cache"]
+    if s["k_scales"] is None:
+        cache.flatten(0, 1)[rows] = x
+        return
+    codes, exponents = _quantise(x.float())
+    cache.view(torch.uint8).flatten(0, 1)[rows] = codes.view(torch.uint8)
+    s[f"{name}_scales"].view(torch.uint8).flatten(0, 1)[rows] = exponents
+
+
+def _plain_read(s, rows, name):
+    """float32 values of these rows of the cache."""
+    cache = s[f"{name}_cache"]
+    if s["k_scales"] is None:
+        return cache.flatten(0, 1)[rows].float()
+    codes = cache.view(torch.uint8).flatten(0, 1)[rows].view(torch.float8_e4m3fn)
+    return _values(codes, s[f"{name}_scales"].view(torch.uint8).flatten(0, 1)[rows])
+
+
+def _plain_attend(s, q, counts, causal):
+    """q [B, L, H, D], of whose rows counts [B] are tokens."""
+    batch, most, heads, head_dim = q.shape
+    heads_kv = s["k_cache"].shape[2]
+    group = heads // heads_kv
+    keys = s["longest"]
+    position = torch.arange(keys, device="cuda")
+    valid = position[None, :] < s["seq_lens"][:, None]  # [B, S]
+    sequence = torch.arange(batch, device="cuda")[:, None].expand(batch, keys)
+    rows = _places(s, sequence, position[None, :].expand(batch, keys))
+    rows = torch.where(valid, rows, 0)
+    k, v = (torch.where(valid[..., None, None], _plain_read(s, rows, t), 0.0) for t in "kv")
+    q = q.float().reshape(batch, most, heads_kv, group, head_dim).permute(0, 2, 1, 3, 4).flatten(2, 3)
+    scores = torch.matmul(q, k.permute(0, 2, 3, 1).contiguous()).mul_(1.0 / math.sqrt(head_dim))
+    scores = scores.reshape(batch, heads_kv, most, group, keys)
+    seen = valid[:, None, :]
+    if causal:
+        last = (s["seq_lens"] - counts)[:, None] + torch.arange(most, device="cuda")[None, :]
+        seen = seen & (position <= last[..., None])  # [B, L, S]
+    scores.masked_fill_(~seen[:, None, :, None, :], -math.inf)
+    top = scores.amax(dim=-1, keepdim=True)
+    top = torch.where(top == -math.inf, 0.0, top)
+    scores.sub_(top).exp_()
+    total = scores.sum(dim=-1, keepdim=True)
+    out = torch.matmul(scores.flatten(2, 3), v.permute(0, 2, 1, 3).contiguous())
+    out = out.reshape(batch, heads_kv, most, group, head_dim)
+    out = torch.where(total > 0, out / total, 0.0)
+    lse = (top + total.log()).squeeze(-1)
+    return (out.permute(0, 2, 1, 3, 4).reshape(batch, most, heads, head_dim).to(s["dtype"]),
+            lse.permute(0, 2, 1, 3).reshape(batch, most, heads))
+
+
+def run(state):
+    if own:
+        return _own(state)
+    s = state
+    if s["op"] in ("write", "read"):
+        sequence, _, position = _new_rows(s)
+        rows = _places(s, sequence, position)
+        if s["op"] == "write":
+            _plain_write(s, rows, "k")
+            _plain_write(s, rows, "v")
+        return tuple(_plain_read(s, rows, t).to(s["dtype"]) for t in "kv")
+    counts = s["cu_seqlens"][1:] - s["cu_seqlens"][:-1]
+    if s["op"] == "attend":
+        sequence, index, _ = _new_rows(s)
+        batch, heads, head_dim = counts.numel(), *s["q"].shape[1:]
+        q = torch.zeros((batch, s["most"], heads, head_dim), device="cuda", dtype=s["dtype"])
+        q[sequence, index] = s["q"]
+        out, lse = _plain_attend(s, q, counts, True)
+        return out[sequence, index], lse[sequence, index]
+    out, lse = _plain_attend(s, s["q"], counts, False)
+    # (decode's log-sum-exps are [B, H])
+    return out, (lse[:, 0] if s["op"] == "decode" else lse)
+
+
+def work(case):
+    """Every input read once and every output written once; the products of the keys that each query
+    row sees."""
+    lens, counts = _sizes(case)
+    heads, heads_kv, head_dim = (case[k] for k in ("heads", "heads_kv", "head_dim"))
+    elem = 2
+    stored = head_dim + 1 if case["cache"] == "e4m3" else head_dim * elem  # bytes of a row
+    tokens = sum(counts)
+    page = PAGES[case["layout"]]
+    table = 4 * sum(-(-n // page) for n in lens) if page else 0
+    if case["op"] == "write":  # the new rows in, into the cache, out of it, and out
+        return {"bytes": 4 * tokens * heads_kv * (head_dim * elem + stored) + table, "flops": 0}
+    if case["op"] == "read":
+        return {"bytes": 2 * tokens * heads_kv * (head_dim * elem + stored) + table, "flops": 0}
+    causal = case["op"] == "attend"
+    pairs = sum(c * n - (c * (c - 1) // 2 if causal else 0) for n, c in zip(lens, counts))
+    keys = sum(n for n, c in zip(lens, counts) if c)
+    nbytes = 2 * keys * heads_kv * stored + tokens * heads * (2 * head_dim * elem + 4) + table
+    return {"bytes": nbytes, "flops": 4 * pairs * heads * head_dim}
+
+
+def _exact_rows(s, name, b, n):
+    """float64 values [n, H_kv, D] of a sequence's first n rows."""
+    cache, scales = s[f"{name}_cache"], s[f"{name}_scales"]
+    if s["tables"] is None:
+        cache = cache[b, :n]
+        scales = None if scales is None else scales[b, :n]
+    else:
+        page = cache.shape[1]
+        blocks = s["tables"][b, : -(-n // page)].tolist()
+        cache = torch.cat([cache[i] for i in blocks])[:n] if n else cache[0, :0]
+        scales = None if scales is None else torch.cat([scales[i].view(torch.uint8) for i in blocks])[:n]
+    if scales is None:
+        return cache.double()
+    return cache.float().double() * torch.exp2(scales.view(torch.uint8).double() - 127.0).unsqueeze(-1)
+
+
+def _exact_round_trip(x):
+    """The values that rows stand for after they were quantised, by the definition of the format: four
+    significant bits, exponents from -6, the scale a power of two."""
+    x = x.double()
+    top = x.abs().amax(dim=-1, keepdim=True)
+    exponent = torch.ceil(torch.log2(torch.where(top > 0, top, 448.0) / 448.0))
+    # (ceil(log2) next to a power of two, put right)
+    exponent = torch.where(top * torch.exp2(1 - exponent) <= 448.0, exponent - 1, exponent)
+    exponent = torch.where(top * torch.exp2(-exponent) > 448.0, exponent + 1, exponent).clamp(-126, 120)
+    y = x * torch.exp2(-exponent)
+    step = torch.exp2((torch.frexp(y)[1].clamp(min=-5) - 4).double())
+    return torch.round(y / step) * step * torch.exp2(exponent)
+
+
+def exact(case, seed):
+    s = prepare(case, seed)
+    lens, counts = _sizes(case)
+    if case["op"] == "write":
+        if case["cache"] == "same":
+            return s["k"].double(), s["v"].double()
+        return tuple(_exact_round_trip(s[t]).to(s["dtype"]).double() for t in "kv")
+    if case["op"] == "read":
+        return tuple(torch.cat([_exact_rows(s, t, b, n) for b, n in enumerate(lens)]) for t in "kv")
+    heads, heads_kv, head_dim = case["heads"], case["heads_kv"], case["head_dim"]
+    group = heads // heads_kv
+    ragged = case["op"] == "attend"
+    q = s["q"] if ragged else s["q"].flatten(0, 1)
+    out = torch.zeros(q.shape, device="cuda", dtype=torch.float64)
+    lse = torch.zeros(q.shape[:2], device="cuda", dtype=torch.float64)
+    start = 0
+    for b, (n, c) in enumerate(zip(lens, counts)):
+        k, v = (_exact_rows(s, t, b, n) for t in "kv")
+        hidden = None
+        if ragged and c:
+            limit = torch.arange(n - c, n, device="cuda").repeat_interleave(group)
+            hidden = torch.arange(n, device="cuda")[None, :] > limit[:, None]
+        for h in range(heads_kv if c else 0):
+            mine = slice(h * group, (h + 1) * group)
+            rows = q[start : start + c, mine].double().reshape(c * group, head_dim)
+            scores = torch.matmul(rows / math.sqrt(head_dim), k[:, h].t().contiguous())
+            if hidden is not None:
+                scores.masked_fill_(hidden, -math.inf)
+            sums = torch.logsumexp(scores, dim=-1)
+            weights = scores.sub_(sums[:, None]).exp_()
+            out[start : start + c, mine] = torch.matmul(weights, v[:, h].contiguous()).reshape(c, group, head_dim)
+            lse[start : start + c, mine] = sums.reshape(c, group)
+        start += c
+    if ragged:
+        return out, lse
+    if case["op"] == "decode":
+        return out.reshape(s["q"].shape), lse
+    return out.reshape(s["q"].shape), lse.reshape(s["q"].shape[:3])
