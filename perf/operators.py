@@ -1,7 +1,7 @@
 """The operators of a served key-value cache that the framework is timed on.
 
 A cache holds every sequence's keys and values, either in the model's type or in 8 bits: e4m3 codes
-with one power-of-two scale (an exponent byte) for each token and KV head. It is a pool of blocks
+with one power-of-two scale (its exponent byte) for each token and KV head. It is a pool of blocks
 with block tables, or one slab per sequence. Four operators work on it:
 
     "write"   new tokens' rows go into the cache, quantised where it holds 8 bits, and the rows are
@@ -220,7 +220,7 @@ def prepare(case, seed):
             codes[~held] = 0x7F
             scales[~held] = 0xFF
             s[f"{name}_cache"] = codes.view(torch.float8_e4m3fn)
-            s[f"{name}_scales"] = scales.view(torch.float8_e8m0fnu)
+            s[f"{name}_scales"] = scales
         else:
             x[~held] = math.nan
             s[f"{name}_cache"] = x
@@ -286,7 +286,7 @@ def _plain_write(s, rows, name):
         return
     codes, exponents = _quantise(x.float())
     cache.view(torch.uint8).flatten(0, 1)[rows] = codes.view(torch.uint8)
-    s[f"{name}_scales"].view(torch.uint8).flatten(0, 1)[rows] = exponents
+    s[f"{name}_scales"].flatten(0, 1)[rows] = exponents
 
 
 def _plain_read(s, rows, name):
@@ -295,7 +295,7 @@ def _plain_read(s, rows, name):
     if s["k_scales"] is None:
         return cache.flatten(0, 1)[rows].float()
     codes = cache.view(torch.uint8).flatten(0, 1)[rows].view(torch.float8_e4m3fn)
-    return _values(codes, s[f"{name}_scales"].view(torch.uint8).flatten(0, 1)[rows])
+    return _values(codes, s[f"{name}_scales"].flatten(0, 1)[rows])
 
 
 def _plain_attend(s, q, counts, causal):
@@ -385,10 +385,10 @@ def _exact_rows(s, name, b, n):
         page = cache.shape[1]
         blocks = s["tables"][b, : -(-n // page)].tolist()
         cache = torch.cat([cache[i] for i in blocks])[:n] if n else cache[0, :0]
-        scales = None if scales is None else torch.cat([scales[i].view(torch.uint8) for i in blocks])[:n]
+        scales = None if scales is None else torch.cat([scales[i] for i in blocks])[:n]
     if scales is None:
         return cache.double()
-    return cache.float().double() * torch.exp2(scales.view(torch.uint8).double() - 127.0).unsqueeze(-1)
+    return cache.float().double() * torch.exp2(scales.double() - 127.0).unsqueeze(-1)
 
 
 def _exact_round_trip(x):
