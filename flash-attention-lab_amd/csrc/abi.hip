@@ -1,6 +1,6 @@
 // The C ABI declared in include/flash_lab_hip.h: argument checks, parameter derivation and
 // kernel launch. Host code only (the kernels live in prefill_fwd.hip, prefill_pp.hip, decode.hip,
-// decode_mfma.hip and smoke.hip).
+// decode_mfma.hip, cache.hip, cached_attn.hip and smoke.hip).
 //
 // The checks restate the reference's op-boundary checks (csrc/common/attn_host.h:18-50,
 // csrc/decode/decode_host.h:18-53, csrc/decode/decode.cu:286-293) on plain pointers and strides;
@@ -524,6 +524,147 @@ int attention_call(const fl_attn_params* p, int num_splits, float* workspace, si
   return FL_OK;
 }
 
+// ---------------------------------------------------------------------------------------------
+// The cache operators (cache.hip, cached_attn.hip).
+
+int cache_elem_bytes(int32_t dtype) { return dtype == FL_DTYPE_E4M3 ? 1 : elem_bytes(dtype); }
+
+// Sizes and types of a cache and of the call's tokens; no pointers.
+int check_cache_shape(const fl_kv_cache& c) {
+  if (c.dtype < FL_DTYPE_BF16 || c.dtype > FL_DTYPE_E4M3)
+    return fail(FL_ERR_UNSUPPORTED, "a cache holds bf16, fp16, fp32 or e4m3");
+  if (c.head_dim != 64 && c.head_dim != 128)
+    return fail(FL_ERR_UNSUPPORTED, fmt("unsupported head_dim %lld", c.head_dim));
+  if (c.batch <= 0 || c.heads_kv <= 0 || c.rows <= 0 || c.outer <= 0 || c.tokens < 0)
+    return fail(FL_ERR_INVALID, "empty input");
+  if (c.block_tables != nullptr) {
+    if (c.max_blocks <= 0) return fail(FL_ERR_INVALID, "block_tables must have at least one block per sequence");
+    if (static_cast<int64_t>(c.max_blocks) * c.rows > INT32_MAX)
+      return fail(FL_ERR_INVALID, "paged cache too long (max_blocks * page_size must fit in int32)");
+  } else if (c.outer != c.batch) {
+    return fail(FL_ERR_INVALID, "batch size mismatch between the cache and the sequences");
+  }
+  if (c.cu_seqlens == nullptr &&
+      (c.tokens_per_seq < 0 || static_cast<int64_t>(c.tokens_per_seq) * c.batch != c.tokens))
+    return fail(FL_ERR_INVALID, "without cu_seqlens every sequence has tokens_per_seq tokens");
+  if (static_cast<int64_t>(c.tokens) * c.heads_kv > INT32_MAX - 256)
+    return fail(FL_ERR_INVALID, "tokens * KV heads too large");
+  return FL_OK;
+}
+
+int check_cache(const fl_kv_cache& c) {
+  if (int rc = check_cache_shape(c)) return rc;
+  if (!c.k || !c.v || !c.seq_lens) return fail(FL_ERR_INVALID, "null tensor pointer");
+  const bool e4m3 = c.dtype == FL_DTYPE_E4M3;
+  if (e4m3 != (c.k_scales != nullptr) || e4m3 != (c.v_scales != nullptr))
+    return fail(FL_ERR_INVALID, "k_scales and v_scales go with an e4m3 cache, and with no other");
+  const int eb = cache_elem_bytes(c.dtype);
+  if (!rows_16_byte(c.k, eb, c.outer, c.k_batch_stride, c.rows, c.k_seq_stride, c.heads_kv, c.k_head_stride))
+    return fail(FL_ERR_INVALID, "k_cache must have 16-byte aligned rows (data pointer and strides)");
+  if (!rows_16_byte(c.v, eb, c.outer, c.v_batch_stride, c.rows, c.v_seq_stride, c.heads_kv, c.v_head_stride))
+    return fail(FL_ERR_INVALID, "v_cache must have 16-byte aligned rows (data pointer and strides)");
+  if (!aligned(c.seq_lens, 4) || (c.cu_seqlens && !aligned(c.cu_seqlens, 4)) ||
+      (c.block_tables && !aligned(c.block_tables, 4)))
+    return fail(FL_ERR_INVALID, "seq_lens, cu_seqlens and block_tables must be 4-byte aligned");
+  return FL_OK;
+}
+
+fl::CacheArgs cache_args(const fl_kv_cache& c) {
+  fl::CacheArgs a{};
+  a.k = static_cast<char*>(c.k);
+  a.v = static_cast<char*>(c.v);
+  a.k_scales = c.k_scales;
+  a.v_scales = c.v_scales;
+  a.seq_lens = c.seq_lens;
+  a.cu_seqlens = c.cu_seqlens;
+  a.block_tables = c.block_tables;
+  a.k_bs = c.k_batch_stride;
+  a.k_ss = c.k_seq_stride;
+  a.k_hs = c.k_head_stride;
+  a.v_bs = c.v_batch_stride;
+  a.v_ss = c.v_seq_stride;
+  a.v_hs = c.v_head_stride;
+  a.ks_bs = c.ks_batch_stride;
+  a.ks_ss = c.ks_seq_stride;
+  a.ks_hs = c.ks_head_stride;
+  a.vs_bs = c.vs_batch_stride;
+  a.vs_ss = c.vs_seq_stride;
+  a.vs_hs = c.vs_head_stride;
+  a.block_tables_stride = c.block_tables_stride;
+  a.batch = c.batch;
+  a.outer = c.outer;
+  a.rows = c.rows;
+  a.heads_kv = c.heads_kv;
+  a.capacity = c.block_tables != nullptr ? c.max_blocks * c.rows : c.rows;
+  a.page_shift = -1;
+  for (int s = 0; s < 31; ++s)
+    if (c.rows == (1 << s)) a.page_shift = s;
+  a.tokens = c.tokens;
+  a.tokens_per_seq = c.tokens_per_seq;
+  return a;
+}
+
+int cache_rows_call(const fl_kv_cache* c, const fl_token_rows* r, bool write, fl_stream_t stream) {
+  if (c == nullptr || r == nullptr) return fail(FL_ERR_INVALID, "null cache parameters");
+  if (int rc = check_cache(*c)) return rc;
+  if (r->dtype != FL_DTYPE_BF16 && r->dtype != FL_DTYPE_F16 && r->dtype != FL_DTYPE_F32)
+    return fail(FL_ERR_UNSUPPORTED, "token rows are bf16, fp16, or fp32");
+  if (c->dtype != FL_DTYPE_E4M3 && c->dtype != r->dtype)
+    return fail(FL_ERR_INVALID, "token rows must have the cache's dtype, unless that is e4m3");
+  if (c->tokens == 0) return FL_OK;
+  if (!r->k || !r->v) return fail(FL_ERR_INVALID, "null tensor pointer");
+  const int eb = elem_bytes(r->dtype);
+  const int64_t outer = c->cu_seqlens ? 1 : c->batch;
+  const int64_t inner = c->cu_seqlens ? c->tokens : c->tokens_per_seq;
+  if (!rows_16_byte(r->k, eb, outer, r->k_batch_stride, inner, r->k_seq_stride, c->heads_kv, r->k_head_stride))
+    return fail(FL_ERR_INVALID, "k must have 16-byte aligned rows (data pointer and strides)");
+  if (!rows_16_byte(r->v, eb, outer, r->v_batch_stride, inner, r->v_seq_stride, c->heads_kv, r->v_head_stride))
+    return fail(FL_ERR_INVALID, "v must have 16-byte aligned rows (data pointer and strides)");
+  fl::TokenRows rows{static_cast<char*>(r->k), static_cast<char*>(r->v),
+                     r->k_batch_stride, r->k_seq_stride, r->k_head_stride,
+                     r->v_batch_stride, r->v_seq_stride, r->v_head_stride};
+  const auto launch = write ? fl::launch_cache_write : fl::launch_cache_read;
+  const hipError_t err = launch(cache_args(*c), rows, decode_dtype(r->dtype), c->dtype == FL_DTYPE_E4M3, c->head_dim,
+                                static_cast<hipStream_t>(stream));
+  if (err != hipSuccess)
+    return fail(FL_ERR_LAUNCH, std::string(write ? "cache write launch: " : "cache read launch: ") + hipGetErrorString(err));
+  return FL_OK;
+}
+
+int check_cached_shape(const fl_cached_attn_params* p) {
+  if (p == nullptr) return fail(FL_ERR_INVALID, "null attention parameters");
+  if (int rc = check_cache_shape(p->cache)) return rc;
+  if (p->dtype != FL_DTYPE_BF16 && p->dtype != FL_DTYPE_F16)
+    return fail(FL_ERR_UNSUPPORTED, "attention_cached takes bf16 or fp16");
+  if (p->cache.dtype != FL_DTYPE_E4M3 && p->cache.dtype != p->dtype)
+    return fail(FL_ERR_INVALID, "the caches must have q's dtype, unless they hold e4m3");
+  if (p->heads <= 0) return fail(FL_ERR_INVALID, "empty input");
+  if (p->heads % p->cache.heads_kv != 0)
+    return fail(FL_ERR_INVALID, "query heads must be a multiple of KV heads");
+  if (static_cast<int64_t>(p->cache.tokens) * p->heads > INT32_MAX - 256)
+    return fail(FL_ERR_INVALID, "tokens * heads too large");
+  if (p->num_splits < 0 || p->num_splits > fl::kMaxSplits)
+    return fail(FL_ERR_INVALID, "num_splits must be in [0, 128]");
+  return FL_OK;
+}
+
+// The kernels' arguments of a checked call, apart from its workspace, and how it is launched.
+int cached_plan(const fl_cached_attn_params* p, int32_t cu_count, fl::CachedAttnArgs& a, fl::CachedPlan& plan) {
+  a.c = cache_args(p->cache);
+  a.heads = p->heads;
+  a.group = p->heads / p->cache.heads_kv;
+  a.causal = p->causal != 0;
+  a.num_splits = p->num_splits;
+  // (Division by the group as in attention_sizes.)
+  a.group_shift = 31;
+  while ((int64_t{1} << (a.group_shift - 31)) < a.group) ++a.group_shift;
+  a.group_mul = static_cast<uint32_t>((uint64_t{1} << a.group_shift) / static_cast<uint32_t>(a.group) + 1);
+  plan = fl::plan_cached_attn(a, p->cache.head_dim, cu_count);
+  if (plan.workgroups > (int64_t{1} << 24))
+    return fail(FL_ERR_INVALID, "tokens * heads * num_splits exceeds the grid limit");
+  return FL_OK;
+}
+
 // The split workspace of fl_decode_noalloc: a file-scope device array, one copy per GPU (each GPU
 // the library runs on holds it until the process ends). In host code `scratch` is a host-side
 // stand-in for the array, not its device address: the address comes from hipGetSymbolAddress,
@@ -733,6 +874,67 @@ int fl_decode_noalloc(const fl_decode_params* p, fl_stream_t stream) {
     if (int rc = scratch_for_current_device(&ws)) return rc;
   }
   return decode_call(p, 0, ws, kScratchBytes, stream);
+}
+
+int fl_cache_write(const fl_kv_cache* cache, const fl_token_rows* rows, fl_stream_t stream) {
+  return cache_rows_call(cache, rows, true, stream);
+}
+
+int fl_cache_read(const fl_kv_cache* cache, const fl_token_rows* rows, fl_stream_t stream) {
+  return cache_rows_call(cache, rows, false, stream);
+}
+
+int fl_cached_attention_plan(const fl_cached_attn_params* p, int32_t cu_count, size_t* workspace_bytes) {
+  if (int rc = check_cached_shape(p)) return rc;
+  if (workspace_bytes == nullptr) return fail(FL_ERR_INVALID, "null output pointer");
+  fl::CachedAttnArgs a{};
+  fl::CachedPlan plan{};
+  if (int rc = cached_plan(p, cu_count, a, plan)) return rc;
+  *workspace_bytes = p->cache.tokens > 0 ? plan.floats * sizeof(float) : 0;
+  return FL_OK;
+}
+
+int fl_cached_attention(const fl_cached_attn_params* p, int32_t cu_count, fl_stream_t stream) {
+  if (int rc = check_cached_shape(p)) return rc;
+  const fl_kv_cache& c = p->cache;
+  if (int rc = check_cache(c)) return rc;
+  if (!valid_scale(p->softmax_scale)) return fail(FL_ERR_INVALID, "softmax_scale must be positive");
+  if (c.tokens == 0) return FL_OK;
+  if (!p->q || !p->o || !p->lse) return fail(FL_ERR_INVALID, "null tensor pointer");
+  const int64_t outer = c.cu_seqlens ? 1 : c.batch;
+  const int64_t inner = c.cu_seqlens ? c.tokens : c.tokens_per_seq;
+  if (!rows_16_byte(p->q, 2, outer, p->q_batch_stride, inner, p->q_seq_stride, p->heads, p->q_head_stride))
+    return fail(FL_ERR_INVALID, "q must have 16-byte aligned rows (data pointer and strides)");
+  if (!rows_16_byte(p->o, 2, outer, p->o_batch_stride, inner, p->o_seq_stride, p->heads, p->o_head_stride))
+    return fail(FL_ERR_INVALID, "o must have 16-byte aligned rows (data pointer and strides)");
+  if (!aligned(p->lse, 4)) return fail(FL_ERR_INVALID, "lse must be 4-byte aligned");
+  fl::CachedAttnArgs a{};
+  fl::CachedPlan plan{};
+  if (int rc = cached_plan(p, cu_count, a, plan)) return rc;
+  a.q = static_cast<const uint16_t*>(p->q);
+  a.o = static_cast<uint16_t*>(p->o);
+  a.lse = p->lse;
+  a.q_bs = p->q_batch_stride;
+  a.q_ss = p->q_seq_stride;
+  a.q_hs = p->q_head_stride;
+  a.o_bs = p->o_batch_stride;
+  a.o_ss = p->o_seq_stride;
+  a.o_hs = p->o_head_stride;
+  a.scale_log2 = static_cast<float>(p->softmax_scale * 1.4426950408889634);
+  if (plan.floats > 0) {
+    if (p->workspace == nullptr || p->workspace_bytes < plan.floats * sizeof(float))
+      return fail(FL_ERR_INVALID,
+                  "attention workspace is missing or smaller than fl_cached_attention_plan reports");
+    if (!aligned(p->workspace, 16)) return fail(FL_ERR_INVALID, "attention workspace must be 16-byte aligned");
+    a.partial_o = p->workspace;
+    a.partial_ml = reinterpret_cast<fl::f32pair*>(a.partial_o + plan.partial_rows * c.head_dim);
+    a.sequence_splits = reinterpret_cast<int2*>(a.partial_ml + plan.partial_rows);
+  }
+  const hipError_t err = fl::launch_cached_attn(a, plan, decode_dtype(p->dtype), c.dtype == FL_DTYPE_E4M3, c.head_dim,
+                                                static_cast<hipStream_t>(stream));
+  if (err != hipSuccess)
+    return fail(FL_ERR_LAUNCH, std::string("cached attention launch: ") + hipGetErrorString(err));
+  return FL_OK;
 }
 
 int fl_smoke_axpy(const float* x, const float* y, float alpha, float* out, int64_t n,

@@ -95,6 +95,54 @@ struct DecodeArgs {
   int2* row_slots;
 };
 
+// A cache and the call's tokens (fl_kv_cache), validated.
+struct CacheArgs {
+  char* k;
+  char* v;
+  uint8_t* k_scales;
+  uint8_t* v_scales;
+  const int32_t* seq_lens;
+  const int32_t* cu_seqlens;    // null: tokens_per_seq each
+  const int32_t* block_tables;  // null: slabs
+  int64_t k_bs, k_ss, k_hs;     // elements, as all strides
+  int64_t v_bs, v_ss, v_hs;
+  int64_t ks_bs, ks_ss, ks_hs;
+  int64_t vs_bs, vs_ss, vs_hs;
+  int64_t block_tables_stride;
+  int batch, outer, rows, heads_kv;
+  int capacity;    // tokens that a sequence can hold
+  int page_shift;  // log2(rows) when it is a power of two, else -1
+  int tokens, tokens_per_seq;
+};
+
+// Source of a cache write, destination of a read.
+struct TokenRows {
+  char* k;
+  char* v;
+  int64_t k_bs, k_ss, k_hs;
+  int64_t v_bs, v_ss, v_hs;
+};
+
+struct CachedAttnArgs {
+  CacheArgs c;
+  const uint16_t* q;
+  uint16_t* o;
+  float* lse;  // [tokens, H]
+  int64_t q_bs, q_ss, q_hs;
+  int64_t o_bs, o_ss, o_hs;
+  int heads, group, causal;
+  float scale_log2;
+  // r / group is (r group_mul) >> group_shift for every r in [0, 2^31).
+  uint32_t group_mul;
+  int group_shift;
+  int num_splits;  // forced, or 0
+  int slots;       // split calls: workgroups that the keys are shared out to at most; 0: no splits
+  int min_tiles;   // fewest key tiles of a split
+  float* partial_o;       // [slot][row of the block][D] unnormalized
+  f32pair* partial_ml;    // [slot][row of the block] (reference point in log2 units or -inf, sum)
+  int2* sequence_splits;  // [B] (splits, first slot) of the sequences with tokens
+};
+
 // How the decode kernels find cache rows: contiguous cache, paged cache with the split's block
 // numbers staged in LDS, or paged cache with the block numbers read from the table in global memory
 // (splits that touch more than kMaxSplitPages blocks).
@@ -159,6 +207,24 @@ hipError_t launch_decode(const DecodeArgs& args, DType dtype, int head_dim, hipS
 // The matrix-core split kernel alone (launch_decode runs it and the merge pass when args.mfma).
 hipError_t launch_decode_mfma_split(const DecodeArgs& args, DType dtype, int head_dim,
                                     hipStream_t stream);
+
+// The cache operators (cache.hip). `rows_dtype`: of the token rows; e4m3: the cache holds codes, else it is
+// of rows_dtype too.
+hipError_t launch_cache_write(const CacheArgs& args, const TokenRows& rows, DType rows_dtype, bool e4m3,
+                              int head_dim, hipStream_t stream);
+hipError_t launch_cache_read(const CacheArgs& args, const TokenRows& rows, DType rows_dtype, bool e4m3,
+                             int head_dim, hipStream_t stream);
+
+// Attention over a cache (cached_attn.hip). The plan fills slots and min_tiles and gives the grid's
+// workgroups and the floats of the workspace (partial_o, then partial_ml, then sequence_splits).
+struct CachedPlan {
+  int64_t workgroups;
+  int64_t partial_rows;  // slots x rows of a block
+  int64_t floats;
+};
+CachedPlan plan_cached_attn(CachedAttnArgs& args, int head_dim, int cu_count);
+hipError_t launch_cached_attn(const CachedAttnArgs& args, const CachedPlan& plan, DType dtype, bool e4m3,
+                              int head_dim, hipStream_t stream);
 
 hipError_t launch_axpy(const float* x, const float* y, float alpha, float* out, int64_t n,
                        hipStream_t stream);

@@ -18,8 +18,10 @@
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/library.h>
 
+#include <optional>
 #include <string>
 #include <tuple>
+#include <utility>
 
 #include "flash_lab_hip.h"
 
@@ -35,6 +37,10 @@ struct Library {
   decltype(&fl_decode_schedule) decode_schedule;
   decltype(&fl_decode) decode;
   decltype(&fl_decode_balanced) decode_balanced;
+  decltype(&fl_cache_write) cache_write;
+  decltype(&fl_cache_read) cache_read;
+  decltype(&fl_cached_attention_plan) cached_attention_plan;
+  decltype(&fl_cached_attention) cached_attention;
   decltype(&fl_last_error) last_error;
 };
 Library lib{};
@@ -226,6 +232,189 @@ Pair paged_decode_op(const Tensor& q, const Tensor& k, const Tensor& v, const Te
   return decode(q, k, v, seq_lens, &block_tables, scale, num_splits, kSplits);
 }
 
+// ---------------------------------------------------------------------------------------------
+// The cache operators: a cache is slabs [B, S_max, H_kv, D] or, with block_tables, a pool of blocks, in the
+// tokens' type or in e4m3 codes with scales. No counterpart in the reference.
+
+using OptTensor = std::optional<Tensor>;
+
+int32_t cache_dtype_code(const Tensor& x) {
+  return x.scalar_type() == at::kFloat8_e4m3fn ? int32_t{FL_DTYPE_E4M3} : dtype_code(x);
+}
+
+// The cache and the call's tokens: `tokens` of them, of B sequences that cu_seqlens parts, or per_seq each
+// without it.
+fl_kv_cache kv_cache(const Tensor& k_cache, const Tensor& v_cache, const OptTensor& k_scales,
+                     const OptTensor& v_scales, const Tensor& seq_lens, const OptTensor& cu_seqlens,
+                     const OptTensor& block_tables, at::ScalarType dtype, int64_t tokens, int64_t per_seq) {
+  check_cuda(k_cache, "k_cache");
+  check_cuda(v_cache, "v_cache");
+  check_cuda(seq_lens, "seq_lens");
+  auto same_device = [&](const Tensor& x, const char* name) {
+    TORCH_CHECK(x.device() == k_cache.device(), name, " is on ", x.device(), ", k_cache on ", k_cache.device());
+  };
+  same_device(v_cache, "v_cache");
+  same_device(seq_lens, "seq_lens");
+  TORCH_CHECK(k_cache.dim() == 4, "caches must be [B, S_max, H_kv, D] or [num_blocks, page_size, H_kv, D]");
+  TORCH_CHECK(k_cache.sizes() == v_cache.sizes(), "k_cache and v_cache must have the same shape");
+  TORCH_CHECK(k_cache.scalar_type() == v_cache.scalar_type(), "k_cache and v_cache must have the same dtype");
+  check_rows(k_cache, "k_cache");
+  check_rows(v_cache, "v_cache");
+  const bool e4m3 = k_cache.scalar_type() == at::kFloat8_e4m3fn;
+  TORCH_CHECK(e4m3 || k_cache.scalar_type() == dtype, "the caches must have the tokens' dtype, or float8_e4m3fn");
+  TORCH_CHECK(e4m3 == k_scales.has_value() && e4m3 == v_scales.has_value(),
+              "k_scales and v_scales go with float8_e4m3fn caches, and with no other");
+  TORCH_CHECK(seq_lens.scalar_type() == at::kInt && seq_lens.dim() == 1 && seq_lens.is_contiguous() &&
+                  seq_lens.size(0) >= 1,
+              "seq_lens must be a contiguous int32 [B]");
+  fl_kv_cache c{};
+  c.k = k_cache.data_ptr();
+  c.v = v_cache.data_ptr();
+  c.seq_lens = seq_lens.const_data_ptr<int32_t>();
+  c.k_batch_stride = k_cache.stride(0), c.k_seq_stride = k_cache.stride(1), c.k_head_stride = k_cache.stride(2);
+  c.v_batch_stride = v_cache.stride(0), c.v_seq_stride = v_cache.stride(1), c.v_head_stride = v_cache.stride(2);
+  c.batch = size32(seq_lens.size(0));
+  c.outer = size32(k_cache.size(0));
+  c.rows = size32(k_cache.size(1));
+  c.heads_kv = size32(k_cache.size(2));
+  c.head_dim = size32(k_cache.size(3));
+  c.dtype = cache_dtype_code(k_cache);
+  c.tokens = size32(tokens);
+  c.tokens_per_seq = size32(per_seq);
+  if (e4m3) {
+    for (const Tensor* s : {&*k_scales, &*v_scales}) {
+      check_cuda(*s, "k_scales and v_scales");
+      same_device(*s, "a scale tensor");
+      TORCH_CHECK(s->scalar_type() == at::kByte && s->sizes() == k_cache.sizes().slice(0, 3),
+                  "k_scales and v_scales must be uint8 of the caches' shape without D");
+    }
+    c.k_scales = static_cast<uint8_t*>(k_scales->data_ptr());
+    c.v_scales = static_cast<uint8_t*>(v_scales->data_ptr());
+    c.ks_batch_stride = k_scales->stride(0), c.ks_seq_stride = k_scales->stride(1);
+    c.vs_batch_stride = v_scales->stride(0), c.vs_seq_stride = v_scales->stride(1);
+    c.ks_head_stride = k_scales->stride(2), c.vs_head_stride = v_scales->stride(2);
+  }
+  if (cu_seqlens) {
+    check_cuda(*cu_seqlens, "cu_seqlens");
+    same_device(*cu_seqlens, "cu_seqlens");
+    TORCH_CHECK(cu_seqlens->scalar_type() == at::kInt && cu_seqlens->dim() == 1 && cu_seqlens->is_contiguous() &&
+                    cu_seqlens->size(0) == seq_lens.size(0) + 1,
+                "cu_seqlens must be a contiguous int32 [B + 1]");
+    c.cu_seqlens = cu_seqlens->const_data_ptr<int32_t>();
+  }
+  if (block_tables) {
+    check_cuda(*block_tables, "block_tables");
+    same_device(*block_tables, "block_tables");
+    TORCH_CHECK(block_tables->scalar_type() == at::kInt && block_tables->dim() == 2 &&
+                    block_tables->size(0) == seq_lens.size(0) && block_tables->size(1) >= 1 &&
+                    block_tables->stride(1) == 1,
+                "block_tables must be int32 [B, max_blocks] with unit stride in its last dimension");
+    c.block_tables = block_tables->const_data_ptr<int32_t>();
+    c.block_tables_stride = block_tables->stride(0);
+    c.max_blocks = size32(block_tables->size(1));
+  } else {
+    TORCH_CHECK(k_cache.size(0) == seq_lens.size(0), "batch size mismatch: the cache has ", k_cache.size(0),
+                ", seq_lens ", seq_lens.size(0));
+  }
+  return c;
+}
+
+// Tokens in all and per sequence of a tensor [tokens, H, D], or [B, S, H, D] without cu_seqlens.
+std::pair<int64_t, int64_t> token_counts(const Tensor& x, const char* name, const Tensor& seq_lens,
+                                         const OptTensor& cu_seqlens) {
+  check_cuda(x, name);
+  check_rows(x, name);
+  if (cu_seqlens) {
+    TORCH_CHECK(x.dim() == 3, name, " must be [tokens, H, D] with cu_seqlens");
+    return {x.size(0), 0};
+  }
+  TORCH_CHECK(x.dim() == 4 && seq_lens.dim() == 1 && x.size(0) == seq_lens.size(0), name,
+              " must be [B, S, H, D] without cu_seqlens");
+  return {x.size(0) * x.size(1), x.size(1)};
+}
+
+// (Ragged tensors have no batch stride.)
+int64_t batch_stride(const Tensor& x) { return x.dim() == 4 ? x.stride(0) : 0; }
+
+fl_token_rows token_rows(const Tensor& k, const Tensor& v, const Tensor& k_cache) {
+  TORCH_CHECK(k.sizes() == v.sizes() && k.scalar_type() == v.scalar_type() && k.device() == v.device(),
+              "k and v must have the same shape, dtype and device");
+  TORCH_CHECK(k.device() == k_cache.device(), "k is on ", k.device(), ", k_cache on ", k_cache.device());
+  TORCH_CHECK(k.scalar_type() == at::kBFloat16 || k.scalar_type() == at::kHalf || k.scalar_type() == at::kFloat,
+              "token rows are bf16, fp16, or fp32");
+  TORCH_CHECK(k_cache.dim() == 4 && k.size(-2) == k_cache.size(2) && k.size(-1) == k_cache.size(3),
+              "token rows and caches must agree on KV heads and head_dim");
+  fl_token_rows r{};
+  r.k = k.data_ptr();
+  r.v = v.data_ptr();
+  r.k_batch_stride = batch_stride(k), r.k_seq_stride = k.stride(-3), r.k_head_stride = k.stride(-2);
+  r.v_batch_stride = batch_stride(v), r.v_seq_stride = v.stride(-3), r.v_head_stride = v.stride(-2);
+  r.dtype = dtype_code(k);
+  return r;
+}
+
+void write_cache(const Tensor& k, const Tensor& v, const Tensor& k_cache, const Tensor& v_cache,
+                 const OptTensor& k_scales, const OptTensor& v_scales, const Tensor& seq_lens,
+                 const OptTensor& cu_seqlens, const OptTensor& block_tables) {
+  const auto [tokens, per_seq] = token_counts(k, "k", seq_lens, cu_seqlens);
+  token_counts(v, "v", seq_lens, cu_seqlens);
+  const fl_token_rows rows = token_rows(k, v, k_cache);
+  const fl_kv_cache c = kv_cache(k_cache, v_cache, k_scales, v_scales, seq_lens, cu_seqlens, block_tables,
+                                 k.scalar_type(), tokens, per_seq);
+  const c10::DeviceGuard guard(k_cache.device());
+  check(lib.cache_write(&c, &rows, current_stream(k_cache)));
+}
+
+Pair read_cache(const Tensor& k_cache, const Tensor& v_cache, const OptTensor& k_scales, const OptTensor& v_scales,
+                const Tensor& seq_lens, const Tensor& cu_seqlens, const OptTensor& block_tables, int64_t num_tokens,
+                at::ScalarType dtype) {
+  TORCH_CHECK(num_tokens >= 0, "num_tokens must not be negative");
+  const fl_kv_cache c = kv_cache(k_cache, v_cache, k_scales, v_scales, seq_lens, cu_seqlens, block_tables, dtype,
+                                 num_tokens, 0);
+  const c10::DeviceGuard guard(k_cache.device());
+  const auto options = k_cache.options().dtype(dtype).memory_format(at::MemoryFormat::Contiguous);
+  Tensor k = at::empty({num_tokens, k_cache.size(2), k_cache.size(3)}, options);
+  Tensor v = at::empty_like(k);
+  const fl_token_rows rows = token_rows(k, v, k_cache);
+  check(lib.cache_read(&c, &rows, current_stream(k_cache)));
+  return {k, v};
+}
+
+Pair attention_cached(const Tensor& q, const Tensor& k_cache, const Tensor& v_cache, const OptTensor& k_scales,
+                      const OptTensor& v_scales, const Tensor& seq_lens, const OptTensor& cu_seqlens,
+                      const OptTensor& block_tables, bool causal, double softmax_scale, int64_t num_splits) {
+  const auto [tokens, per_seq] = token_counts(q, "q", seq_lens, cu_seqlens);
+  TORCH_CHECK(q.scalar_type() == at::kBFloat16 || q.scalar_type() == at::kHalf, "attention_cached takes bf16 or fp16");
+  TORCH_CHECK(q.device() == k_cache.device(), "q is on ", q.device(), ", k_cache on ", k_cache.device());
+  TORCH_CHECK(k_cache.dim() == 4 && k_cache.size(3) == q.size(-1), "q and the caches must agree on head_dim");
+  TORCH_CHECK(0 <= num_splits && num_splits <= 128, "num_splits must be in [0, 128]");
+  const c10::DeviceGuard guard(q.device());
+  Tensor o = at::empty(q.sizes(), q.options().memory_format(at::MemoryFormat::Contiguous));
+  Tensor lse = at::empty(q.sizes().slice(0, q.dim() - 1), q.options().dtype(at::kFloat).memory_format(at::MemoryFormat::Contiguous));
+  fl_cached_attn_params p{};
+  p.cache = kv_cache(k_cache, v_cache, k_scales, v_scales, seq_lens, cu_seqlens, block_tables, q.scalar_type(), tokens,
+                     per_seq);
+  p.q = q.const_data_ptr();
+  p.o = o.data_ptr();
+  p.lse = lse.data_ptr<float>();
+  p.q_batch_stride = batch_stride(q), p.q_seq_stride = q.stride(-3), p.q_head_stride = q.stride(-2);
+  p.o_batch_stride = batch_stride(o), p.o_seq_stride = o.stride(-3), p.o_head_stride = o.stride(-2);
+  p.heads = size32(q.size(-2));
+  p.causal = causal;
+  p.dtype = dtype_code(q);
+  p.num_splits = static_cast<int32_t>(num_splits);
+  p.softmax_scale = softmax_scale;
+  const int32_t cus = cu_count(q);
+  check(lib.cached_attention_plan(&p, cus, &p.workspace_bytes));
+  Tensor workspace;
+  if (p.workspace_bytes > 0) {
+    workspace = at::empty({static_cast<int64_t>(p.workspace_bytes / sizeof(float))}, lse.options());
+    p.workspace = workspace.data_ptr<float>();
+  }
+  check(lib.cached_attention(&p, cus, current_stream(q)));
+  return {o, lse};
+}
+
 // The ops have no gradient. With inputs that require one, the outputs are part of the graph and a
 // backward through them raises; otherwise the call goes straight on below autograd.
 template <typename... Args>
@@ -246,6 +435,7 @@ struct NoGradient {
     }
   };
   static bool requires_grad(const Tensor& x) { return x.requires_grad(); }
+  static bool requires_grad(const OptTensor& x) { return x && x->requires_grad(); }
   template <typename T>
   static bool requires_grad(const T&) {
     return false;
@@ -290,6 +480,43 @@ FL_DECODE_AUTOGRAD(decode_inplace)
 FL_PAGED_AUTOGRAD(decode_splitkv_paged)
 FL_PAGED_AUTOGRAD(decode_inplace_paged)
 
+using CachedAttention = NoGradient<const Tensor&, const Tensor&, const Tensor&, const OptTensor&, const OptTensor&,
+                                   const Tensor&, const OptTensor&, const OptTensor&, bool, double, int64_t>;
+FL_AUTOGRAD(CachedAttention, attention_cached,
+            (const Tensor& q, const Tensor& k, const Tensor& v, const OptTensor& ks, const OptTensor& vs,
+             const Tensor& lens, const OptTensor& cu, const OptTensor& tables, bool causal, double scale, int64_t n),
+            ("attention_cached", op, q, k, v, ks, vs, lens, cu, tables, causal, scale, n))
+using ReadCache = NoGradient<const Tensor&, const Tensor&, const OptTensor&, const OptTensor&, const Tensor&,
+                             const Tensor&, const OptTensor&, int64_t, at::ScalarType>;
+FL_AUTOGRAD(ReadCache, read_cache,
+            (const Tensor& k, const Tensor& v, const OptTensor& ks, const OptTensor& vs, const Tensor& lens,
+             const Tensor& cu, const OptTensor& tables, int64_t n, at::ScalarType dtype),
+            ("read_cache", op, k, v, ks, vs, lens, cu, tables, n, dtype))
+
+// A write gives nothing that a backward could start from, so rows that require a gradient would lose it
+// without a word: they are refused.
+void write_cache_autograd(const Tensor& k, const Tensor& v, const Tensor& k_cache, const Tensor& v_cache,
+                          const OptTensor& k_scales, const OptTensor& v_scales, const Tensor& seq_lens,
+                          const OptTensor& cu_seqlens, const OptTensor& block_tables) {
+  static const auto op = c10::Dispatcher::singleton().findSchemaOrThrow("flash_lab::write_cache", "")
+                             .typed<decltype(write_cache)>();
+  TORCH_CHECK(!at::GradMode::is_enabled() || !(k.requires_grad() || v.requires_grad() || k_cache.requires_grad() ||
+                                               v_cache.requires_grad()),
+              "write_cache has no gradient: pass detached rows and caches, or call it under torch.no_grad()");
+  {
+    at::AutoDispatchBelowADInplaceOrView below;
+    op.call(k, v, k_cache, v_cache, k_scales, v_scales, seq_lens, cu_seqlens, block_tables);
+  }
+  // A graph that saved one of these for its backward then says that it was changed.
+  auto changed = [](const Tensor& x) {
+    if (!x.is_inference()) x.unsafeGetTensorImpl()->bump_version();
+  };
+  changed(k_cache);
+  changed(v_cache);
+  if (k_scales) changed(*k_scales);
+  if (v_scales) changed(*v_scales);
+}
+
 }  // namespace
 
 // The reference's schemas, verbatim (csrc/bindings.cpp:9-41); the paged forms, which the reference
@@ -309,6 +536,16 @@ TORCH_LIBRARY_FRAGMENT(flash_lab, m) {
   def("decode_inplace", decode);
   def("decode_splitkv_paged", paged);
   def("decode_inplace_paged", paged);
+  def("attention_cached",
+      "(Tensor q, Tensor k_cache, Tensor v_cache, Tensor? k_scales, Tensor? v_scales, Tensor seq_lens,"
+      " Tensor? cu_seqlens, Tensor? block_tables, bool causal, float softmax_scale, int num_splits)"
+      " -> (Tensor, Tensor)");
+  def("write_cache",
+      "(Tensor k, Tensor v, Tensor(a!) k_cache, Tensor(b!) v_cache, Tensor(c!)? k_scales, Tensor(d!)? v_scales,"
+      " Tensor seq_lens, Tensor? cu_seqlens, Tensor? block_tables) -> ()");
+  def("read_cache",
+      "(Tensor k_cache, Tensor v_cache, Tensor? k_scales, Tensor? v_scales, Tensor seq_lens, Tensor cu_seqlens,"
+      " Tensor? block_tables, int num_tokens, ScalarType dtype) -> (Tensor, Tensor)");
 }
 
 TORCH_LIBRARY_IMPL(flash_lab, CUDA, m) {
@@ -318,6 +555,9 @@ TORCH_LIBRARY_IMPL(flash_lab, CUDA, m) {
   m.impl("decode_inplace", &decode_op<false>);
   m.impl("decode_splitkv_paged", &paged_decode_op<true>);
   m.impl("decode_inplace_paged", &paged_decode_op<false>);
+  m.impl("attention_cached", &attention_cached);
+  m.impl("write_cache", &write_cache);
+  m.impl("read_cache", &read_cache);
 }
 
 TORCH_LIBRARY_IMPL(flash_lab, Autograd, m) {
@@ -327,16 +567,25 @@ TORCH_LIBRARY_IMPL(flash_lab, Autograd, m) {
   m.impl("decode_inplace", &decode_inplace_autograd);
   m.impl("decode_splitkv_paged", &decode_splitkv_paged_autograd);
   m.impl("decode_inplace_paged", &decode_inplace_paged_autograd);
+  m.impl("attention_cached", &attention_cached_autograd);
+  m.impl("write_cache", &write_cache_autograd);
+  m.impl("read_cache", &read_cache_autograd);
 }
 
 // The addresses of the library's functions, in this order; once, before the first call of an op.
 extern "C" void fl_torch_bind(void* attention_plan, void* attention_fwd_split, void* decode_plan,
-                              void* decode_schedule, void* decode, void* decode_balanced, void* last_error) {
+                              void* decode_schedule, void* decode, void* decode_balanced, void* cache_write,
+                              void* cache_read, void* cached_attention_plan, void* cached_attention,
+                              void* last_error) {
   lib.attention_plan = reinterpret_cast<decltype(lib.attention_plan)>(attention_plan);
   lib.attention_fwd_split = reinterpret_cast<decltype(lib.attention_fwd_split)>(attention_fwd_split);
   lib.decode_plan = reinterpret_cast<decltype(lib.decode_plan)>(decode_plan);
   lib.decode_schedule = reinterpret_cast<decltype(lib.decode_schedule)>(decode_schedule);
   lib.decode = reinterpret_cast<decltype(lib.decode)>(decode);
   lib.decode_balanced = reinterpret_cast<decltype(lib.decode_balanced)>(decode_balanced);
+  lib.cache_write = reinterpret_cast<decltype(lib.cache_write)>(cache_write);
+  lib.cache_read = reinterpret_cast<decltype(lib.cache_read)>(cache_read);
+  lib.cached_attention_plan = reinterpret_cast<decltype(lib.cached_attention_plan)>(cached_attention_plan);
+  lib.cached_attention = reinterpret_cast<decltype(lib.cached_attention)>(cached_attention);
   lib.last_error = reinterpret_cast<decltype(lib.last_error)>(last_error);
 }

@@ -10,6 +10,14 @@ registers, under torch.ops.flash_lab, ops with the reference's names and schemas
         (Tensor q, Tensor k_cache, Tensor v_cache, Tensor seq_lens, float softmax_scale,
          int num_splits) -> (Tensor, Tensor)
     decode_splitkv_paged / decode_inplace_paged: the same with block_tables after seq_lens
+    attention_cached(Tensor q, Tensor k_cache, Tensor v_cache, Tensor? k_scales, Tensor? v_scales,
+                     Tensor seq_lens, Tensor? cu_seqlens, Tensor? block_tables, bool causal,
+                     float softmax_scale, int num_splits) -> (Tensor, Tensor)
+    write_cache(Tensor k, Tensor v, Tensor(a!) k_cache, Tensor(b!) v_cache, Tensor(c!)? k_scales,
+                Tensor(d!)? v_scales, Tensor seq_lens, Tensor? cu_seqlens, Tensor? block_tables) -> ()
+    read_cache(Tensor k_cache, Tensor v_cache, Tensor? k_scales, Tensor? v_scales, Tensor seq_lens,
+               Tensor cu_seqlens, Tensor? block_tables, int num_tokens, ScalarType dtype)
+        -> (Tensor, Tensor)
     smoke_axpy(Tensor x, Tensor y, float alpha) -> Tensor
     mma_tile_test(Tensor a, Tensor b, bool trans_b) -> Tensor
 
@@ -36,7 +44,7 @@ LIB_NAME = "libflash_lab_hip.so"
 LIB_PATH = Path(os.environ.get("FLASH_LAB_HIP_LIB", Path(__file__).with_name(LIB_NAME)))
 
 ERR_WORKSPACE = 4  # enum fl_status
-DTYPE_CODES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
+DTYPE_CODES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2, torch.float8_e4m3fn: 3}
 
 
 class AttnParams(ctypes.Structure):
@@ -102,6 +110,49 @@ class DecodeParams(ctypes.Structure):
     ]
 
 
+class KvCache(ctypes.Structure):
+    """fl_kv_cache of include/flash_lab_hip.h."""
+
+    _fields_ = [
+        *[(name, ctypes.c_void_p) for name in
+          ("k", "v", "k_scales", "v_scales", "seq_lens", "cu_seqlens", "block_tables")],
+        *[(f"{t}_{s}_stride", ctypes.c_int64) for t in ("k", "v", "ks", "vs") for s in ("batch", "seq", "head")],
+        ("block_tables_stride", ctypes.c_int64),
+        *[(name, ctypes.c_int32) for name in
+          ("batch", "outer", "rows", "max_blocks", "heads_kv", "head_dim", "dtype", "tokens", "tokens_per_seq")],
+    ]
+
+
+class TokenRows(ctypes.Structure):
+    """fl_token_rows of include/flash_lab_hip.h."""
+
+    _fields_ = [
+        ("k", ctypes.c_void_p),
+        ("v", ctypes.c_void_p),
+        *[(f"{t}_{s}_stride", ctypes.c_int64) for t in ("k", "v") for s in ("batch", "seq", "head")],
+        ("dtype", ctypes.c_int32),
+    ]
+
+
+class CachedAttnParams(ctypes.Structure):
+    """fl_cached_attn_params of include/flash_lab_hip.h."""
+
+    _fields_ = [
+        ("cache", KvCache),
+        ("q", ctypes.c_void_p),
+        ("o", ctypes.c_void_p),
+        ("lse", ctypes.c_void_p),
+        *[(f"{t}_{s}_stride", ctypes.c_int64) for t in ("q", "o") for s in ("batch", "seq", "head")],
+        ("heads", ctypes.c_int32),
+        ("causal", ctypes.c_int32),
+        ("dtype", ctypes.c_int32),
+        ("num_splits", ctypes.c_int32),
+        ("softmax_scale", ctypes.c_double),
+        ("workspace", ctypes.c_void_p),
+        ("workspace_bytes", ctypes.c_size_t),
+    ]
+
+
 # Every symbol include/flash_lab_hip.h declares, with its ctypes signature.
 SIGNATURES = {
     "fl_attention_fwd": (ctypes.c_int, [ctypes.POINTER(AttnParams), ctypes.c_void_p]),
@@ -153,6 +204,16 @@ SIGNATURES = {
     ),
     "fl_decode": (ctypes.c_int, [ctypes.POINTER(DecodeParams), ctypes.c_void_p]),
     "fl_decode_noalloc": (ctypes.c_int, [ctypes.POINTER(DecodeParams), ctypes.c_void_p]),
+    "fl_cache_write": (ctypes.c_int, [ctypes.POINTER(KvCache), ctypes.POINTER(TokenRows), ctypes.c_void_p]),
+    "fl_cache_read": (ctypes.c_int, [ctypes.POINTER(KvCache), ctypes.POINTER(TokenRows), ctypes.c_void_p]),
+    "fl_cached_attention_plan": (
+        ctypes.c_int,
+        [ctypes.POINTER(CachedAttnParams), ctypes.c_int32, ctypes.POINTER(ctypes.c_size_t)],
+    ),
+    "fl_cached_attention": (
+        ctypes.c_int,
+        [ctypes.POINTER(CachedAttnParams), ctypes.c_int32, ctypes.c_void_p],
+    ),
     "fl_smoke_axpy": (
         ctypes.c_int,
         [
@@ -205,7 +266,8 @@ LIB = load_library()
 TORCH_LIB_PATH = Path(__file__).with_name("libflash_lab_torch.so")
 # The library functions that fl_torch_bind takes, in its order.
 TORCH_BOUND = ("fl_attention_plan", "fl_attention_fwd_split", "fl_decode_plan", "fl_decode_schedule", "fl_decode",
-               "fl_decode_balanced", "fl_last_error")
+               "fl_decode_balanced", "fl_cache_write", "fl_cache_read", "fl_cached_attention_plan",
+               "fl_cached_attention", "fl_last_error")
 
 
 def load_torch_ops(path: Path = TORCH_LIB_PATH) -> ctypes.CDLL:
@@ -452,6 +514,9 @@ OPS = (
     "decode_inplace",
     "decode_splitkv_paged",
     "decode_inplace_paged",
+    "attention_cached",
+    "write_cache",
+    "read_cache",
     "smoke_axpy",
     "mma_tile_test",
 )

@@ -28,7 +28,12 @@ extern "C" {
 /* A hipStream_t. NULL is the null stream of the current device. */
 typedef void* fl_stream_t;
 
-enum fl_dtype { FL_DTYPE_BF16 = 0, FL_DTYPE_F16 = 1, FL_DTYPE_F32 = 2 };
+enum fl_dtype {
+  FL_DTYPE_BF16 = 0,
+  FL_DTYPE_F16 = 1,
+  FL_DTYPE_F32 = 2,
+  FL_DTYPE_E4M3 = 3 /* caches only (fl_kv_cache): 8-bit codes with a scale per row */
+};
 
 enum fl_status {
   FL_OK = 0,
@@ -189,6 +194,107 @@ int fl_decode(const fl_decode_params* p, fl_stream_t stream);
  * array's previous contents never reach an output.
  */
 int fl_decode_noalloc(const fl_decode_params* p, fl_stream_t stream);
+
+/*
+ * A key-value cache that new tokens are written into and attended to (the cache operators below; no
+ * counterpart in the reference, whose callers write their caches with torch). k and v are slabs
+ * [B, rows, H_kv, D], or, with block_tables, pools [outer, rows, H_kv, D] of `outer` blocks of `rows`
+ * rows each, as in fl_decode_params. Strides are in elements; D has unit stride.
+ *
+ * dtype is the elements' type. With FL_DTYPE_E4M3 they are e4m3 codes (the OCP format with NaN and
+ * without infinities, largest value 448), and k_scales and v_scales [B or outer, rows, H_kv] hold the
+ * exponent byte of every row's scale: code c of a row stands for c 2^(byte - 127). Bytes 1 to 254 are
+ * scales; the operators write 1 to 247.
+ *
+ * Sequence b has seq_lens[b] tokens, of which the last n_b are the call's (written, read or
+ * attending): tokens cu_seqlens[b] .. cu_seqlens[b + 1] - 1 of the call's ragged [tokens, ...] tensors,
+ * or, where cu_seqlens is NULL, tokens_per_seq tokens each of tensors [B, tokens_per_seq, ...]. Token i
+ * of them is at position seq_lens[b] - n_b + i. seq_lens, cu_seqlens and block_tables are int32 on the
+ * device and never read by the host. A sequence holds at most `rows` tokens, max_blocks * rows in a pool.
+ * Whatever the device arrays hold, nothing is read or written outside the tensors.
+ */
+typedef struct fl_kv_cache {
+  void* k;
+  void* v;
+  uint8_t* k_scales; /* FL_DTYPE_E4M3 only, else NULL */
+  uint8_t* v_scales;
+  const int32_t* seq_lens;
+  const int32_t* cu_seqlens;   /* [B + 1], or NULL */
+  const int32_t* block_tables; /* [B, max_blocks], or NULL: slabs */
+  int64_t k_batch_stride, k_seq_stride, k_head_stride; /* batch: of a slab or of a block */
+  int64_t v_batch_stride, v_seq_stride, v_head_stride;
+  int64_t ks_batch_stride, ks_seq_stride, ks_head_stride;
+  int64_t vs_batch_stride, vs_seq_stride, vs_head_stride;
+  int64_t block_tables_stride;
+  int32_t batch, outer, rows, max_blocks, heads_kv, head_dim;
+  int32_t dtype;          /* enum fl_dtype */
+  int32_t tokens;         /* of the call, all sequences together (rows behind the last one included) */
+  int32_t tokens_per_seq; /* where cu_seqlens is NULL */
+} fl_kv_cache;
+
+/*
+ * Rows of the call's tokens, [tokens, H_kv, D] (or [B, tokens_per_seq, H_kv, D]: seq strides step from
+ * token to token, batch strides from sequence to sequence): the source of a write, the destination of a
+ * read. dtype is BF16, F16 or F32, and the cache's own unless that is E4M3.
+ */
+typedef struct fl_token_rows {
+  void* k;
+  void* v;
+  int64_t k_batch_stride, k_seq_stride, k_head_stride;
+  int64_t v_batch_stride, v_seq_stride, v_head_stride;
+  int32_t dtype;
+} fl_token_rows;
+
+/*
+ * Writes the tokens' rows into the cache. An E4M3 cache gets, for a row with largest finite magnitude
+ * m, the scale 2^e with the least e in [-126, 120] for which m 2^-e <= 448 (e = 0 for m = 0), and the
+ * codes of x 2^-e rounded to nearest even; infinities and NaN become NaN. Magnitudes are held first to
+ * the largest that the rows' type holds after the rounding too: 61,440 in F16, 1.875 2^127 in BF16 and
+ * F32. Tokens whose
+ * position is outside the cache, or whose table entry is outside the pool, are not written, and neither
+ * are rows of `rows` that belong to no sequence. Two sequences' tokens must not share a row of the
+ * cache (its content is then undefined).
+ */
+int fl_cache_write(const fl_kv_cache* cache, const fl_token_rows* rows, fl_stream_t stream);
+
+/*
+ * Reads the tokens' rows back as the values they stand for, rounded to rows->dtype where that cannot
+ * hold them. Rows of tokens that the cache does not hold (a position outside it), and rows of no
+ * sequence, are zeroed; table entries outside the pool are clamped.
+ */
+int fl_cache_read(const fl_kv_cache* cache, const fl_token_rows* rows, fl_stream_t stream);
+
+/*
+ * Attention of the call's tokens to their sequences' caches, which hold the tokens' own rows already.
+ * q and o are [tokens, H, D] (or [B, tokens_per_seq, H, D]) in `dtype`, BF16 or F16, which is the
+ * cache's too unless that is E4M3; lse [tokens, H] fp32, contiguous. Token i of sequence b sees its
+ * first seq_lens[b] keys, and with `causal` of those the ones at positions up to its own. A token
+ * that sees no key, and rows that belong to no sequence, get o = 0 and lse = -inf. Lengths are clamped to
+ * the cache and table entries to the pool. Probabilities, and codes times scales, are rounded to `dtype`
+ * for the matrix cores.
+ */
+typedef struct fl_cached_attn_params {
+  fl_kv_cache cache;
+  const void* q;
+  void* o;
+  float* lse;
+  int64_t q_batch_stride, q_seq_stride, q_head_stride;
+  int64_t o_batch_stride, o_seq_stride, o_head_stride;
+  int32_t heads, causal, dtype;
+  int32_t num_splits; /* key splits of every row, in [1, 128], or 0: the library's choice */
+  double softmax_scale;
+  float* workspace; /* 16-byte aligned, at least what fl_cached_attention_plan reports */
+  size_t workspace_bytes;
+} fl_cached_attn_params;
+
+/* Workspace of a call; host-only, touches no device, reads only sizes, dtypes and num_splits. */
+int fl_cached_attention_plan(const fl_cached_attn_params* p, int32_t cu_count, size_t* workspace_bytes);
+
+/*
+ * Results are bitwise reproducible for the same call, lengths and cu_count; a token's last bits can
+ * depend on the other sequences' lengths unless num_splits is given.
+ */
+int fl_cached_attention(const fl_cached_attn_params* p, int32_t cu_count, fl_stream_t stream);
 
 /* out = alpha * x + y over n fp32 elements (reference csrc/common/smoke.cu:12-45). */
 int fl_smoke_axpy(const float* x, const float* y, float alpha, float* out, int64_t n,
