@@ -20,7 +20,10 @@ Unwritten rows of a cache hold NaN, as memory that nobody has cleared may.
     lengths   of the sequences with the new tokens: all `longest`, or spread evenly from 1/B of it
 """
 
+import functools
 import math
+import sys
+from pathlib import Path
 
 import torch
 
@@ -236,15 +239,19 @@ def prepare(case, seed):
     return s
 
 
-def _own(s):
-    import sys
-    from pathlib import Path
-
+@functools.cache
+def _package():
+    """The framework, imported once, as a program does."""
     package = str(Path.cwd() / "flash-attention-lab_amd")
     if package not in sys.path:
         sys.path.insert(0, package)
     import flash_lab
 
+    return flash_lab
+
+
+def _own(s):
+    flash_lab = _package()
     cache = dict(block_tables=s["tables"], k_scales=s["k_scales"], v_scales=s["v_scales"])
     if s["op"] == "write":
         flash_lab.write_cache(s["k"], s["v"], s["k_cache"], s["v_cache"], s["seq_lens"],
