@@ -136,7 +136,8 @@ struct CachedAttnArgs {
   uint32_t group_mul;
   int group_shift;
   int num_splits;  // forced, or 0
-  int slots;       // split calls: workgroups that the keys are shared out to at most; 0: no splits
+  int slots;       // workgroups that run at once, where keys may be split; 0: no splits
+  int max_rounds;  // of slots workgroups each
   int min_tiles;   // fewest key tiles of a split
   float* partial_o;       // [slot][row of the block][D] unnormalized
   f32pair* partial_ml;    // [slot][row of the block] (reference point in log2 units or -inf, sum)
@@ -218,6 +219,7 @@ hipError_t launch_cache_read(const CacheArgs& args, const TokenRows& rows, DType
 // Attention over a cache (cached_attn.hip). The plan fills slots and min_tiles and gives the grid's
 // workgroups and the floats of the workspace (partial_o, then partial_ml, then sequence_splits).
 struct CachedPlan {
+  bool narrow, wide;  // whether sequences can have at most 32 rows, and more
   int64_t workgroups;
   int64_t partial_rows;  // slots x rows of a block
   int64_t floats;

@@ -71,13 +71,10 @@ def test_more_sequences_than_lanes(batch):
     check_attention(out, lse, q, cache, counts)
 
 
-@pytest.mark.parametrize("types", TYPES, ids=list(TYPES))
+@pytest.mark.parametrize("dtype", HALF, ids=["bf16", "fp16"])
 @pytest.mark.parametrize("page", [0, 16, 64])
 @pytest.mark.parametrize("heads,heads_kv,head_dim", [(32, 8, 128), (8, 8, 64), (64, 4, 128), (3, 1, 64)])
-def test_decode_over_a_cache(types, page, heads, heads_kv, head_dim):
-    dtype, quantized = TYPES[types]
-    if not quantized:
-        pytest.skip("decode over a cache in q's type has its own tests")
+def test_decode_over_8_bits(dtype, page, heads, heads_kv, head_dim):
     gen = torch.Generator(device="cuda").manual_seed(4)
     lens = [1, 700, 64, 2049]
     cache = make_cache(lens, 2100, heads_kv, head_dim, dtype, True, page, gen)
@@ -284,11 +281,11 @@ def test_refused_types():
     gen = torch.Generator(device="cuda").manual_seed(18)
     cache = make_cache([40], 48, 2, 64, torch.bfloat16, True, 16, gen)
     for dtype in (torch.float32, torch.float64):
-        with pytest.raises(ValueError, match="is not one of"):
+        with pytest.raises(ValueError, match="no available implementation supports"):
             flash_lab.decode(torch.zeros(1, 1, 4, 64, device="cuda", dtype=dtype), **cache)
     wide = make_cache([40], 48, 2, 64, torch.float32, False, 16, gen)
     with pytest.raises(ValueError, match="is not one of"):
-        flash_lab.attention_cached(torch.zeros(1, 1, 4, 64, device="cuda"), **wide)
+        flash_lab.attention_cached(torch.zeros(1, 1, 4, 64, device="cuda"), impl="cached_mma", **wide)
     with pytest.raises(ValueError, match="one device"):
         flash_lab.attention_cached(torch.zeros(1, 1, 4, 64, device="cuda", dtype=torch.bfloat16),
                                    **dict(cache, seq_lens=cache["seq_lens"].cpu()))
