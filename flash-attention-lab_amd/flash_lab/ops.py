@@ -311,6 +311,11 @@ def decode(
     return (out, lse) if return_lse else out
 
 
+# The native ops check their arguments themselves, and a call of one costs less than the checks here: so the
+# cache operators call the op first, and find out what was wrong (and raise as the other entry points do)
+# when it refuses. Under torch.compile, where the ops are not run, the checks come first.
+
+
 def _decode_quantized(q, k_cache, v_cache, seq_lens, block_tables, softmax_scale, impl, num_splits, return_lse,
                       k_scales, v_scales):
     """decode() over a cache in 8 bits: attention_cached with one token per sequence."""
@@ -320,28 +325,27 @@ def _decode_quantized(q, k_cache, v_cache, seq_lens, block_tables, softmax_scale
         raise ValueError(f"impl {impl!r} cannot run a cache in 8 bits; choose 'auto' or 'splitkv'")
     if not isinstance(q, torch.Tensor):
         raise TypeError(f"q must be a torch.Tensor, got {type(q).__name__}")
-    if q.dim() == 4 and q.shape[1] != 1:
+    rank = q.dim()
+    if rank == 4 and q.shape[1] != 1:
         raise ValueError(f"decode takes one query token per sequence, got q {tuple(q.shape)}")
-    if q.dim() not in (3, 4):
+    if rank not in (3, 4):
         raise ValueError(f"q must be [B, 1, H, D] or [B, H, D], got shape {tuple(q.shape)}")
     if num_splits is not None and num_splits < 1:
         raise ValueError(f"num_splits must be positive, got {num_splits}")
-    q4 = q if q.dim() == 4 else q.unsqueeze(1)
-    out, lse = _attention_cached(q4, k_cache, v_cache, seq_lens, None, block_tables, k_scales, v_scales, True,
-                                 softmax_scale, "auto", num_splits or 0)
-    out = out if q.dim() == 4 else out.squeeze(1)
+    out, lse = _attention_cached(q if rank == 4 else q.unsqueeze(1), k_cache, v_cache, seq_lens, None, block_tables,
+                                 k_scales, v_scales, True, softmax_scale, "auto", num_splits or 0)
+    out = out if rank == 4 else out.squeeze(1)
     return (out, lse.squeeze(1)) if return_lse else out
 
 
-def _attention_cached(q, k_cache, v_cache, seq_lens, cu_seqlens, block_tables, k_scales, v_scales, causal,
-                      softmax_scale, impl, num_splits):
+def _check_attention_cached(q, k_cache, v_cache, seq_lens, cu_seqlens, block_tables, k_scales, v_scales,
+                            softmax_scale, impl) -> None:
     cache = check_cache(k_cache, v_cache, seq_lens, block_tables, k_scales, v_scales, cu_seqlens)
     check_token_rows("q", q, cache, k_cache, cu_seqlens)
     check_query_heads(q.shape[-2], cache.heads_kv)
-    scale = 1.0 / math.sqrt(cache.head_dim) if softmax_scale is None else softmax_scale
-    if not scale > 0:
-        raise ValueError(f"softmax_scale must be positive, got {scale}")
-    spec = _select(
+    if softmax_scale is not None and not softmax_scale > 0:
+        raise ValueError(f"softmax_scale must be positive, got {softmax_scale}")
+    _select(
         CACHED_IMPLS,
         impl,
         q.device,
@@ -351,8 +355,20 @@ def _attention_cached(q, k_cache, v_cache, seq_lens, cu_seqlens, block_tables, k
         ),
         lambda s: s.unsupported_reason(cache, q.dtype),
     )
-    return _OVERLOADS[spec.op](q, k_cache, v_cache, k_scales, v_scales, seq_lens, cu_seqlens, block_tables,
-                               causal, scale, num_splits)
+
+
+def _attention_cached(q, k_cache, v_cache, seq_lens, cu_seqlens, block_tables, k_scales, v_scales, causal,
+                      softmax_scale, impl, num_splits):
+    checked = (q, k_cache, v_cache, seq_lens, cu_seqlens, block_tables, k_scales, v_scales, softmax_scale, impl)
+    if impl not in ("auto", "cached_mma") or torch.compiler.is_compiling():
+        _check_attention_cached(*checked)
+    try:
+        scale = 1.0 / math.sqrt(q.shape[-1]) if softmax_scale is None else softmax_scale
+        return _OVERLOADS["attention_cached"](q, k_cache, v_cache, k_scales, v_scales, seq_lens, cu_seqlens,
+                                              block_tables, causal, scale, num_splits)
+    except Exception:
+        _check_attention_cached(*checked)
+        raise
 
 
 def attention_cached(
@@ -391,20 +407,42 @@ def attention_cached(
     return (out, lse) if return_lse else out
 
 
-def _cache_op(name: str, device: torch.device):
+def _check_cache_op(name: str, cache: CacheShape, dtype: torch.dtype, device: torch.device) -> None:
+    if dtype not in _DECODE_DTYPES:
+        raise TypeError(f"token rows must be one of {_DECODE_DTYPES}, got {dtype}")
+    if cache.head_dim not in _DIMS:
+        raise ValueError(f"head_dim {cache.head_dim} is not one of {_DIMS}")
     if device.type != "cuda":
         raise ValueError(f"flash_lab kernels take CUDA tensors, got device {device}")
     if name not in _BUILT_OPS:
         missing = "" if HAS_EXTENSION else f" (the HIP extension did not load: {EXTENSION_ERROR})"
         raise RuntimeError(f"{name} is not available in this build{missing}")
-    return _OVERLOADS[name]
 
 
-def _check_cache_types(cache: CacheShape, dtype: torch.dtype) -> None:
-    if dtype not in _DECODE_DTYPES:
-        raise TypeError(f"token rows must be one of {_DECODE_DTYPES}, got {dtype}")
-    if cache.head_dim not in _DIMS:
-        raise ValueError(f"head_dim {cache.head_dim} is not one of {_DIMS}")
+def _check_write_cache(k, v, k_cache, v_cache, seq_lens, cu_seqlens, block_tables, k_scales, v_scales) -> None:
+    cache = check_cache(k_cache, v_cache, seq_lens, block_tables, k_scales, v_scales, cu_seqlens)
+    for name, x in (("k", k), ("v", v)):
+        check_token_rows(name, x, cache, k_cache, cu_seqlens)
+        if x.shape[-2] != cache.heads_kv:
+            raise ValueError(f"{name} has {x.shape[-2]} heads, the cache has {cache.heads_kv}")
+    if k.shape != v.shape or k.dtype != v.dtype:
+        raise ValueError(f"k and v must have the same shape and dtype, got {tuple(k.shape)} {k.dtype} and "
+                         f"{tuple(v.shape)} {v.dtype}")
+    _check_cache_op("write_cache", cache, k.dtype, k.device)
+
+
+def _check_read_cache(k_cache, v_cache, seq_lens, cu_seqlens, num_tokens, block_tables, k_scales, v_scales,
+                      dtype) -> None:
+    cache = check_cache(k_cache, v_cache, seq_lens, block_tables, k_scales, v_scales, cu_seqlens)
+    if cu_seqlens is None:
+        raise TypeError("cu_seqlens must be a torch.Tensor, got NoneType")
+    if num_tokens < 0:
+        raise ValueError(f"num_tokens must not be negative, got {num_tokens}")
+    if dtype is None:
+        dtype = torch.bfloat16 if cache.quantized else k_cache.dtype
+    if not cache.quantized and dtype != k_cache.dtype:
+        raise TypeError(f"a cache of {k_cache.dtype} is read in its own dtype, got {dtype}")
+    _check_cache_op("read_cache", cache, dtype, k_cache.device)
 
 
 def write_cache(
@@ -433,17 +471,14 @@ def write_cache(
     Tokens whose position is outside the cache, or whose table entry is outside the pool, are not written.
     Sequences must not write to a block that they share (its rows would hold a mixture).
     """
-    cache = check_cache(k_cache, v_cache, seq_lens, block_tables, k_scales, v_scales, cu_seqlens)
-    for name, x in (("k", k), ("v", v)):
-        check_token_rows(name, x, cache, k_cache, cu_seqlens)
-        if x.shape[-2] != cache.heads_kv:
-            raise ValueError(f"{name} has {x.shape[-2]} heads, the cache has {cache.heads_kv}")
-    if k.shape != v.shape or k.dtype != v.dtype:
-        raise ValueError(f"k and v must have the same shape and dtype, got {tuple(k.shape)} {k.dtype} and "
-                         f"{tuple(v.shape)} {v.dtype}")
-    _check_cache_types(cache, k.dtype)
-    _cache_op("write_cache", k.device)(k, v, k_cache, v_cache, k_scales, v_scales, seq_lens, cu_seqlens,
-                                       block_tables)
+    checked = (k, v, k_cache, v_cache, seq_lens, cu_seqlens, block_tables, k_scales, v_scales)
+    if torch.compiler.is_compiling():
+        _check_write_cache(*checked)
+    try:
+        _OVERLOADS["write_cache"](k, v, k_cache, v_cache, k_scales, v_scales, seq_lens, cu_seqlens, block_tables)
+    except Exception:
+        _check_write_cache(*checked)
+        raise
 
 
 def read_cache(
@@ -465,15 +500,14 @@ def read_cache(
     gives `dtype` (bf16 by default; values that fp16 cannot hold are rounded to it), any other its own.
     Rows behind the last sequence, and rows of positions that the cache does not have, are zero.
     """
-    cache = check_cache(k_cache, v_cache, seq_lens, block_tables, k_scales, v_scales, cu_seqlens)
-    if cu_seqlens is None:
-        raise TypeError("cu_seqlens must be a torch.Tensor, got NoneType")
-    if num_tokens < 0:
-        raise ValueError(f"num_tokens must not be negative, got {num_tokens}")
-    if dtype is None:
-        dtype = torch.bfloat16 if cache.quantized else k_cache.dtype
-    if not cache.quantized and dtype != k_cache.dtype:
-        raise TypeError(f"a cache of {k_cache.dtype} is read in its own dtype, got {dtype}")
-    _check_cache_types(cache, dtype)
-    return _cache_op("read_cache", k_cache.device)(k_cache, v_cache, k_scales, v_scales, seq_lens, cu_seqlens,
-                                                   block_tables, num_tokens, dtype)
+    checked = (k_cache, v_cache, seq_lens, cu_seqlens, num_tokens, block_tables, k_scales, v_scales, dtype)
+    if torch.compiler.is_compiling():
+        _check_read_cache(*checked)
+    try:
+        if dtype is None:
+            dtype = torch.bfloat16 if k_scales is not None else k_cache.dtype
+        return _OVERLOADS["read_cache"](k_cache, v_cache, k_scales, v_scales, seq_lens, cu_seqlens, block_tables,
+                                        num_tokens, dtype)
+    except Exception:
+        _check_read_cache(*checked)
+        raise
