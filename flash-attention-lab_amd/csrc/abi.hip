@@ -1,6 +1,6 @@
 // The C ABI declared in include/flash_lab_hip.h: argument checks, parameter derivation and
 // kernel launch. Host code only (the kernels live in prefill_fwd.hip, prefill_pp.hip, decode.hip,
-// decode_mfma.hip, cache.hip, cached_attn.hip and smoke.hip).
+// decode_mfma.hip, cache.hip, cached_*.hip and smoke.hip).
 //
 // The checks restate the reference's op-boundary checks (csrc/common/attn_host.h:18-50,
 // csrc/decode/decode_host.h:18-53, csrc/decode/decode.cu:286-293) on plain pointers and strides;
@@ -659,8 +659,9 @@ int cached_plan(const fl_cached_attn_params* p, int32_t cu_count, fl::CachedAttn
   a.group_shift = 31;
   while ((int64_t{1} << (a.group_shift - 31)) < a.group) ++a.group_shift;
   a.group_mul = static_cast<uint32_t>((uint64_t{1} << a.group_shift) / static_cast<uint32_t>(a.group) + 1);
-  plan = fl::plan_cached_attn(a, p->cache.head_dim, cu_count);
-  if (plan.workgroups > (int64_t{1} << 24))
+  plan = fl::plan_cached_attn(a, p->cache.head_dim, p->cache.dtype == FL_DTYPE_E4M3, cu_count);
+  a.wide_partials = plan.wide_partials;
+  if (plan.narrow.workgroups > (int64_t{1} << 24) || plan.wide.workgroups > (int64_t{1} << 24))
     return fail(FL_ERR_INVALID, "tokens * heads * num_splits exceeds the grid limit");
   return FL_OK;
 }

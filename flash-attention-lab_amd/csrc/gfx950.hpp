@@ -213,6 +213,17 @@ __device__ __forceinline__ float sum_halves(float x) {
   return __uint_as_float(r[0]) + __uint_as_float(r[1]);
 }
 
+// The same over lanes l, l ^ 16, l ^ 32 and l ^ 48: v_permlane16_swap exchanges the odd rows of 16 lanes of one
+// register with the even rows of another.
+__device__ __forceinline__ float max_quarters(float x) {
+  const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return max_halves(max2_f32(__uint_as_float(r[0]), __uint_as_float(r[1])));
+}
+__device__ __forceinline__ float sum_quarters(float x) {
+  const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return sum_halves(__uint_as_float(r[0]) + __uint_as_float(r[1]));
+}
+
 // f(integral_constant<int, i>) for i = I .. N - 1, unrolled at compile time.
 template <int I, int N, typename F>
 __device__ __forceinline__ void static_for(F&& f) {

@@ -136,11 +136,15 @@ struct CachedAttnArgs {
   uint32_t group_mul;
   int group_shift;
   int num_splits;  // forced, or 0
+  // Of the kind of sequences that a kernel runs (cached.hpp):
   int slots;       // workgroups that run at once, where keys may be split; 0: no splits
   int max_rounds;  // of slots workgroups each
   int min_tiles;   // fewest key tiles of a split
-  float* partial_o;       // [slot][row of the block][D] unnormalized
-  f32pair* partial_ml;    // [slot][row of the block] (reference point in log2 units or -inf, sum)
+  // Partials: [slot][row of the block], the narrow sequences' slots first, the wide ones' from row
+  // wide_partials on.
+  int64_t wide_partials;
+  float* partial_o;       // [D] unnormalized
+  f32pair* partial_ml;    // (reference point in log2 units or -inf, sum)
   int2* sequence_splits;  // [B] (splits, first slot) of the sequences with tokens
 };
 
@@ -216,17 +220,27 @@ hipError_t launch_cache_write(const CacheArgs& args, const TokenRows& rows, DTyp
 hipError_t launch_cache_read(const CacheArgs& args, const TokenRows& rows, DType rows_dtype, bool e4m3,
                              int head_dim, hipStream_t stream);
 
-// Attention over a cache (cached_attn.hip). The plan fills slots and min_tiles and gives the grid's
-// workgroups and the floats of the workspace (partial_o, then partial_ml, then sequence_splits).
+// Attention over a cache (cached_attn.hip): how a call is launched, and the floats of its workspace
+// (partial_o, then partial_ml, then sequence_splits).
 struct CachedPlan {
-  bool narrow, wide;  // whether sequences can have at most 32 rows, and more
-  int64_t workgroups;
-  int64_t partial_rows;  // slots x rows of a block
-  int64_t floats;
+  struct Part {
+    int64_t workgroups, partials;  // of the grid, slots of partials
+    int slots, max_rounds, min_tiles;
+  };
+  Part narrow, wide;  // workgroups 0: there are none of the kind
+  int most_rows;      // of a sequence
+  bool many_splits;   // few rows
+  int64_t wide_partials, partial_rows, floats;
 };
-CachedPlan plan_cached_attn(CachedAttnArgs& args, int head_dim, int cu_count);
+CachedPlan plan_cached_attn(const CachedAttnArgs& args, int head_dim, bool e4m3, int cu_count);
 hipError_t launch_cached_attn(const CachedAttnArgs& args, const CachedPlan& plan, DType dtype, bool e4m3,
                               int head_dim, hipStream_t stream);
+// Its two kernels (cached_narrow.hip, cached_wide.hip), and how many workgroups of the first a CU holds.
+int cached_narrow_resident(int head_dim, bool e4m3, bool ragged, int most_rows);
+hipError_t launch_cached_narrow(const CachedAttnArgs& args, const CachedPlan& plan, DType dtype, bool e4m3,
+                                int head_dim, hipStream_t stream);
+hipError_t launch_cached_wide(const CachedAttnArgs& args, int64_t workgroups, DType dtype, bool e4m3, int head_dim,
+                              hipStream_t stream);
 
 hipError_t launch_axpy(const float* x, const float* y, float alpha, float* out, int64_t n,
                        hipStream_t stream);
