@@ -899,6 +899,17 @@ int fl_cached_attention(const fl_cached_attn_params* p, int32_t cu_count, fl_str
   if (int rc = check_cached_shape(p)) return rc;
   const fl_kv_cache& c = p->cache;
   if (int rc = check_cache(c)) return rc;
+  // The kernels step between rows and between a pool's blocks by 32-bit strides.
+  auto fits = [&](int64_t block, int64_t row) {
+    const int64_t most = (int64_t{1} << 32) / cache_elem_bytes(c.dtype) - 1;
+    return (c.rows == 1 || (row >= 0 && row <= most)) &&
+           (c.block_tables == nullptr || c.outer == 1 || (block >= 0 && block <= most));
+  };
+  if (!fits(c.k_batch_stride, c.k_seq_stride) || !fits(c.v_batch_stride, c.v_seq_stride))
+    return fail(FL_ERR_INVALID, "k_cache or v_cache stride too large (4 GiB between rows or blocks)");
+  if (c.dtype == FL_DTYPE_E4M3 &&
+      (!fits(c.ks_batch_stride, c.ks_seq_stride) || !fits(c.vs_batch_stride, c.vs_seq_stride)))
+    return fail(FL_ERR_INVALID, "k_scales or v_scales stride too large (4 GiB between rows or blocks)");
   if (!valid_scale(p->softmax_scale)) return fail(FL_ERR_INVALID, "softmax_scale must be positive");
   if (c.tokens == 0) return FL_OK;
   if (!p->q || !p->o || !p->lse) return fail(FL_ERR_INVALID, "null tensor pointer");

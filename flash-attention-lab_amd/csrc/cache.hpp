@@ -76,6 +76,9 @@ __device__ __forceinline__ Token find_token(const CacheArgs& c, int token) {
 struct Place {
   int outer, row;
 };
+__device__ __forceinline__ int row_in_block(const CacheArgs& c, int position) {
+  return c.page_shift >= 0 ? position & (c.rows - 1) : position % c.rows;
+}
 __device__ __forceinline__ Place place(const CacheArgs& c, int b, int position) {
   if (c.block_tables == nullptr) return Place{b, position};
   const int page = c.page_shift >= 0 ? position >> c.page_shift : position / c.rows;

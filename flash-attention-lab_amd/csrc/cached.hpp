@@ -1,5 +1,6 @@
 // Pieces shared by the kernels of attention over a cache (cached_attn.hip: plan and merge; cached_narrow.hip:
-// sequences with few rows; cached_wide.hip: the others): the rows of a sequence, the items that the
+// sequences with few rows; cached_pp.hip and cached_wide.hip: the
+// others, at head_dim 128 and 64): the rows of a sequence, the items that the
 // workgroups of a kernel share out, and the offsets of cache rows.
 #pragma once
 
@@ -15,13 +16,15 @@ namespace cached {
 // Kinds of sequences, by their rows (tokens x query heads of a KV head).
 enum Kind { kNarrow, kWide };
 constexpr int kNarrowRows = 48;  // most rows of a narrow sequence
-constexpr int kWideRows = 128;   // rows of a block of a wide sequence
 constexpr int kKeys = 64;        // keys of a tile: splits are whole tiles
 constexpr int kStartTiles = 4;   // tiles that starting and ending an item costs as much as
 constexpr int kMaxRounds = 3;
-__host__ __device__ __forceinline__ constexpr int block_rows(Kind kind) {
-  return kind == kNarrow ? kNarrowRows : kWideRows;
+// Rows of a block.
+__host__ __device__ __forceinline__ constexpr int block_rows(Kind kind, int head_dim) {
+  return kind == kNarrow ? kNarrowRows : head_dim == 128 ? 256 : 128;
 }
+// Workgroups of the wide kernel per CU.
+constexpr int wide_resident(int head_dim) { return head_dim == 128 ? 1 : 2; }
 
 namespace {
 
@@ -56,11 +59,11 @@ struct Item {
 struct Load {
   int blocks, tiles;
 };
-template <Kind kKind>
+template <Kind kKind, int D>
 __device__ __forceinline__ Load load_of(const CachedAttnArgs& a, const Sequence& s) {
   const int rows = s.count * a.group;
   const bool mine = (rows <= kNarrowRows) == (kKind == kNarrow);
-  return Load{mine ? (rows + block_rows(kKind) - 1) / block_rows(kKind) : 0, (s.len + kKeys - 1) / kKeys};
+  return Load{mine ? (rows + block_rows(kKind, D) - 1) / block_rows(kKind, D) : 0, (s.len + kKeys - 1) / kKeys};
 }
 
 // The items of a kernel, over the sequences of its kind: sequence b has blocks_b splits_b H_kv of them, with splits_b = ceil(tiles_b / share). a.slots
@@ -69,7 +72,7 @@ __device__ __forceinline__ Load load_of(const CachedAttnArgs& a, const Sequence&
 // share for which no more than r slots items result. Within a chunk of 64 sequences longer items come
 // first where there is more than one round, so that the last ones to start are short. Lane l holds sequence
 // 64 i + l of chunk i; chunks behind the first are read again in every pass.
-template <Kind kKind>
+template <Kind kKind, int D>
 __device__ __forceinline__ bool find_item(const CachedAttnArgs& a, int id, Item& item) {
   const int lane = __lane_id();
   const int batch = a.c.batch;
@@ -79,11 +82,11 @@ __device__ __forceinline__ bool find_item(const CachedAttnArgs& a, int id, Item&
     return s;
   };
   const Sequence first = sequence_at(lane);
-  const Load first_load = load_of<kKind>(a, first);
+  const Load first_load = load_of<kKind, D>(a, first);
   // f(blocks, tiles) summed over all sequences.
   auto sum = [&](auto f) {
     auto total = f(first_load);
-    for (int base = 64; base < batch; base += 64) total += f(load_of<kKind>(a, sequence_at(base + lane)));
+    for (int base = 64; base < batch; base += 64) total += f(load_of<kKind, D>(a, sequence_at(base + lane)));
     return wave_sum(total);
   };
   // Sequences that overlap (cu_seqlens does not ascend) could have more items than the grid and the
@@ -134,7 +137,7 @@ __device__ __forceinline__ bool find_item(const CachedAttnArgs& a, int id, Item&
   int before_slot = 0;  // slots of earlier chunks
   for (int base = 0; base < batch; base += 64) {
     const Sequence s = base == 0 ? first : sequence_at(base + lane);
-    const Load l = load_of<kKind>(a, s);
+    const Load l = load_of<kKind, D>(a, s);
     const int splits = splits_of(l);
     const int items = l.blocks * splits * a.c.heads_kv;
     const int slots = splits > 1 ? items : 0;
@@ -186,14 +189,31 @@ struct Piece {
   static constexpr int kElems = 16 / kElem;
   static constexpr int kPerRow = D / kElems;
 };
-// Where a tensor's rows lie: bytes, or scales. A row's offset is worked out by one lane for all that move
-// its pieces (two 64-bit products, which the pieces' lanes would repeat).
+// Where the rows of one sequence and KV head lie in a tensor (bytes, or scales): `base` and the strides between
+// blocks (0 in a slab) and between rows, in bytes that fit 32 bits (checked on the host), so that an offset is
+// two 32-bit products. It is worked out by one lane for all that move the row's pieces.
 struct RowSpace {
-  int64_t outer_stride, row_stride;
-  __device__ __forceinline__ int64_t offset(const CacheArgs& c, const cache::Place& p) const {
-    return min(max(p.outer, 0), c.outer - 1) * outer_stride + p.row * row_stride;
+  const char* base;
+  uint32_t block_stride, row_stride;
+  __device__ __forceinline__ uint64_t offset(const CacheArgs& c, const cache::Place& p) const {
+    const uint32_t block = static_cast<uint32_t>(min(max(p.outer, 0), c.outer - 1));
+    return static_cast<uint64_t>(block) * block_stride + static_cast<uint64_t>(static_cast<uint32_t>(p.row)) * row_stride;
   }
 };
+__device__ __forceinline__ RowSpace row_space(const CacheArgs& c, const void* tensor, int b, int hkv, int64_t bs,
+                                              int64_t ss, int64_t hs, int elem) {
+  const bool slab = c.block_tables == nullptr;
+  return RowSpace{static_cast<const char*>(tensor) + (hkv * hs + (slab ? b * bs : 0)) * elem,
+                  slab ? 0u : static_cast<uint32_t>(bs * elem), static_cast<uint32_t>(ss * elem)};
+}
+// The spaces of K's (or V's) rows and of their scales.
+__device__ __forceinline__ RowSpace rows_of(const CacheArgs& c, bool v, int b, int hkv, int elem) {
+  return v ? row_space(c, c.v, b, hkv, c.v_bs, c.v_ss, c.v_hs, elem) : row_space(c, c.k, b, hkv, c.k_bs, c.k_ss, c.k_hs, elem);
+}
+__device__ __forceinline__ RowSpace scales_of(const CacheArgs& c, bool v, int b, int hkv) {
+  return v ? row_space(c, c.v_scales, b, hkv, c.vs_bs, c.vs_ss, c.vs_hs, 1)
+           : row_space(c, c.k_scales, b, hkv, c.ks_bs, c.ks_ss, c.ks_hs, 1);
+}
 
 // The merge of partials and what they leave: (reference point, sum) of a row. A sum of zero means that no key
 // was seen; a NaN stays one.

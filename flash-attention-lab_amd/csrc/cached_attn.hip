@@ -9,7 +9,7 @@
 //
 // Lengths are known on the device only. Sequences with few rows (tokens x heads of a group) are bound by
 // reading the cache and run on cached_narrow.hip, those with many by the matrix cores and run on
-// cached_wide.hip; without cu_seqlens the host knows which it is, and only that kernel is launched.
+// cached_pp.hip (head_dim 128) or cached_wide.hip (64); without cu_seqlens the host knows which it is, and only that kernel is launched.
 // Every workgroup of either derives the same list of items from the lengths (find_item, cached.hpp) and
 // takes the one of its own number; the grid is an upper bound from the sizes. Where the items are few, keys
 // are split over several workgroups, and a last kernel, here, merges the partials in order.
@@ -26,13 +26,13 @@ struct Partials {
   int splits;
   int64_t first, step;  // rows of the workspace
 };
-__device__ __forceinline__ Partials partials_of(const CachedAttnArgs& a, const cache::Token& t, int head) {
+__device__ __forceinline__ Partials partials_of(const CachedAttnArgs& a, const cache::Token& t, int head, int head_dim) {
   const int2 info = a.sequence_splits[t.b];
   const int hkv = head / a.group;
   const int rows = t.count * a.group;
   const int r = t.index * a.group + head - hkv * a.group;
   const Kind kind = rows <= kNarrowRows ? kNarrow : kWide;
-  const int per_block = block_rows(kind);
+  const int per_block = block_rows(kind, head_dim);
   const int blocks = (rows + per_block - 1) / per_block;
   const int block = r / per_block;
   const int64_t slot = info.y + (static_cast<int64_t>(blocks - 1 - block) * a.c.heads_kv + hkv) * info.x;
@@ -56,7 +56,7 @@ __global__ void __launch_bounds__(kThreads) cached_merge_kernel(const CachedAttn
   const int head = static_cast<int>(row - static_cast<int64_t>(token) * a.heads);
   const cache::Token t = cache::find_token<kGroups == 1 ? kLanes : 64>(a.c, token);
   if (at >= all || t.b < 0) return;
-  const Partials p = partials_of(a, t, head);
+  const Partials p = partials_of(a, t, head, D);
   const int n = p.splits;
   if (n <= 1) return;
   const int d = threadIdx.x % kLanes;
@@ -159,17 +159,18 @@ CachedPlan plan_cached_attn(const CachedAttnArgs& args, int head_dim, bool e4m3,
   if (ragged || per_seq <= kNarrowRows) {
     const int64_t least = ragged ? 0 : c.batch * int64_t{c.heads_kv};
     plan.narrow = plan_part(args, least, c.batch * int64_t{c.heads_kv},
-                            cus * cached_narrow_resident(head_dim, e4m3, ragged, plan.most_rows), 2);
+                            cus * cached_narrow_resident(head_dim, e4m3, plan.most_rows), 2);
   }
   if (plan.most_rows > kNarrowRows) {
-    const int64_t blocks = (per_seq + kWideRows - 1) / kWideRows * c.batch;
+    const int64_t wide_rows = block_rows(kWide, head_dim);
+    const int64_t blocks = (per_seq + wide_rows - 1) / wide_rows * c.batch;
     const int64_t least = ragged ? 0 : blocks * c.heads_kv;
-    const int64_t most = (ragged ? rows / kWideRows + (c.batch < rows / kNarrowRows + 1 ? c.batch : rows / kNarrowRows + 1)
+    const int64_t most = (ragged ? rows / wide_rows + (c.batch < rows / kNarrowRows + 1 ? c.batch : rows / kNarrowRows + 1)
                                  : blocks) * c.heads_kv;
-    plan.wide = plan_part(args, least, most, 2 * cus, 4);
+    plan.wide = plan_part(args, least, most, wide_resident(head_dim) * cus, 4);
   }
   plan.wide_partials = plan.narrow.partials * kNarrowRows;
-  plan.partial_rows = plan.wide_partials + plan.wide.partials * kWideRows;
+  plan.partial_rows = plan.wide_partials + plan.wide.partials * block_rows(kWide, head_dim);
   if (plan.partial_rows > 0) plan.floats = plan.partial_rows * (head_dim + 2) + 2 * static_cast<int64_t>(c.batch);
   // One workgroup per row pays while the rows are about as few as the CUs and their splits many.
   plan.many_splits = static_cast<int64_t>(c.tokens) * args.heads <= 8 * cus;

@@ -96,7 +96,7 @@ __device__ __forceinline__ void narrow_item(const CachedAttnArgs& a, const Item&
 
   char* work = smem + kQBytes<D, kCols>;
   char* tile = work + wave * kTileBytes<D>;
-  int64_t* offsets = reinterpret_cast<int64_t*>(work + kWaves * kTileBytes<D>) + wave * 64;
+  uint64_t* offsets = reinterpret_cast<uint64_t*>(work + kWaves * kTileBytes<D>) + wave * 64;
 
   // Q^T, the B operand: lane (n, g) holds row 16 c + n, dims step_dim(ks, g) .. + 7.
   const int64_t q_base = a.c.cu_seqlens ? seq.start * a.q_ss : item.b * a.q_bs;
@@ -125,18 +125,17 @@ __device__ __forceinline__ void narrow_item(const CachedAttnArgs& a, const Item&
   // loads its scale.
   const int load_row = lane / P::kPerRow;
   const int load_piece = lane % P::kPerRow;
-  const char* kp = a.c.k + item.hkv * a.c.k_hs * P::kElem + 16 * load_piece;
-  const char* vp = a.c.v + item.hkv * a.c.v_hs * P::kElem + 16 * load_piece;
-  const RowSpace space{(half ? a.c.v_bs : a.c.k_bs) * P::kElem, (half ? a.c.v_ss : a.c.k_ss) * P::kElem};
-  const RowSpace scale_space = half ? RowSpace{a.c.vs_bs, a.c.vs_ss} : RowSpace{a.c.ks_bs, a.c.ks_ss};
-  const uint8_t* my_scales = half ? a.c.v_scales + item.hkv * a.c.vs_hs : a.c.k_scales + item.hkv * a.c.ks_hs;
+  const RowSpace space = rows_of(a.c, half != 0, item.b, item.hkv, P::kElem);
+  const RowSpace scale_space = scales_of(a.c, half != 0, item.b, item.hkv);
+  const char* kp = rows_of(a.c, false, item.b, item.hkv, P::kElem).base + 16 * load_piece;
+  const char* vp = rows_of(a.c, true, item.b, item.hkv, P::kElem).base + 16 * load_piece;
   auto first_key = [&](int i) { return (begin + kWaves * i) * kTileKeys; };
   auto find = [&](int i) { return cache::place(a.c, item.b, min(first_key(i) + (lane & 31), last)); };
   u32x4 k[kPieces], v[kPieces];
   uint32_t byte = 0;
   auto load = [&](const cache::Place& p) __attribute__((always_inline)) {
     offsets[lane] = space.offset(a.c, p);
-    if constexpr (kE4M3) byte = my_scales[scale_space.offset(a.c, p)];
+    if constexpr (kE4M3) byte = static_cast<uint8_t>(scale_space.base[scale_space.offset(a.c, p)]);
 #pragma unroll
     for (int j = 0; j < kPieces; ++j) {
       k[j] = load16_stream(kp + offsets[load_row + j * kRowStep]);
@@ -343,7 +342,7 @@ __device__ __forceinline__ void clear_unowned(const CachedAttnArgs& a) {
 // head_dim 128 does not fit the 128 registers of a fourth: 25 of them spilled, 162 us against 94 for 8 sequences of
 // 32K keys in e4m3, and 105 with two.)
 template <int D, bool kE4M3, int kCols>
-constexpr int kResident = kCols > 1 ? 2 : D == 128 ? 3 : 4;
+constexpr int kResident = kCols > 1 || (D == 128 && !kE4M3) ? 2 : D == 128 ? 3 : 4;
 
 // kCols: column blocks of the largest sequence. With kMixed (ragged batches) sequences of one block run
 // the one-block form.
@@ -354,7 +353,7 @@ __global__ void __launch_bounds__(kThreads)
   __shared__ __attribute__((aligned(16))) char smem[kQBytes<D, kCols> + kWorkBytes<D>];
   clear_unowned<D>(a);
   Item item;
-  if (!find_item<kNarrow>(a, blockIdx.x, item)) return;
+  if (!find_item<kNarrow, D>(a, blockIdx.x, item)) return;
   if (item.first && threadIdx.x == 0 && a.sequence_splits != nullptr)
     a.sequence_splits[item.b] = int2{item.splits, item.first_slot};
   if (kMixed && item.seq.count * a.group <= 16) {
@@ -391,9 +390,8 @@ hipError_t launch_typed(const CachedAttnArgs& args, const CachedPlan& plan, bool
 }  // namespace
 }  // namespace cached
 
-int cached_narrow_resident(int head_dim, bool e4m3, bool ragged, int most_rows) {
-  using namespace cached;
-  if (most_rows > 16) return 2;
+int cached_narrow_resident(int head_dim, bool e4m3, int most_rows) {
+  if (most_rows > 16 || (head_dim == 128 && !e4m3)) return 2;
   return head_dim == 128 ? 3 : 4;
 }
 

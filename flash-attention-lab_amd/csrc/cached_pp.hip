@@ -1,0 +1,509 @@
+// Attention over a cache for sequences with many rows at head_dim 128 (fl_cached_attention, cached.hpp): chunks
+// of prompts, bound by the matrix cores. The arithmetic, lane layouts and phases are those of the prefill
+// kernel (prefill_pp.hip): 8 waves of 32 rows, two to a SIMD in two groups that take turns, one group's
+// MFMAs running beside the other's softmax, one barrier per tile of 64 keys. What differs is where keys
+// come from and how the work is found:
+//
+//  * Rows may lie anywhere (a pool's blocks of any size). Group 0 moves K, group 1 V, 16 rows a wave, in its
+//    MFMA phase, between the MFMAs: one lane works out a row's address, the lanes that move its 16-byte
+//    pieces get it by a lane permute. In period m they ask for tile m + 2, so a load has a whole period (about
+//    2,000 cycles) to come back. Rows in the tokens' type go straight into LDS; codes go through registers,
+//    and a period later become the tokens' type (a pair per instruction, scale included) and go into LDS, once
+//    per workgroup.
+//  * A workgroup has one item, a share of a block's tiles (cached.hpp), and the rows of all query heads of
+//    a KV head.
+#include "cached.hpp"
+#include "prefill_pp.hpp"
+
+namespace fl {
+namespace cached {
+namespace {
+
+using prefill::acc_key;
+using prefill::k_lane_offset;
+using prefill::kKeyBlockBytes;
+using prefill::kKeyStepBytes;
+using prefill::kMoveSlack;
+using prefill::kTileElems;
+using prefill::max_of;
+using prefill::p_frag;
+using prefill::tile_offset;
+using prefill::v_frag_at;
+using prefill::v_lane_offset;
+using prefill::pp::phase_barrier;
+
+constexpr int D = 128;
+constexpr int kWaves = 8;
+constexpr int kThreads = 64 * kWaves;
+constexpr int kWaveRows = 32;
+constexpr int kRows = kWaves * kWaveRows;
+static_assert(kRows == block_rows(kWide, D), "a wave per 32 rows");
+// LDS slots for K and for V: in period m the tiles m - 1 (V), m and m + 1, and in the tokens' type m + 2, which
+// loads bring in (codes arrive in a place of their own).
+template <bool kE4M3>
+constexpr int kStagesOf = kE4M3 ? 3 : 4;
+constexpr int kAhead = 2;   // fragments read ahead of their MFMAs
+
+// What V's rows behind a sequence's last one are read as.
+__device__ const u32x4 zero_row[D * 2 / 16] = {};
+
+template <typename Tag, bool kE4M3>
+__global__ void __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2, 2)))
+    cached_pp_kernel(const CachedAttnArgs a) {
+  using E = Elem<Tag>;
+  using P = Piece<D, kE4M3>;
+  constexpr int kStages = kStagesOf<kE4M3>;
+  constexpr int kTile = kTileElems<D>;
+  constexpr int kSlotBytes = 2 * kTile;
+  constexpr int kVRingBytes = kStages * kSlotBytes;
+  constexpr int kCodeBytes = kE4M3 ? 16 * D : 0;  // a wave's rows of a tile, as codes
+  constexpr int kCodesAt = 2 * kVRingBytes;
+  __shared__ __attribute__((aligned(16))) uint16_t smem[(kCodesAt + 2 * kWaves * kCodeBytes) / 2];
+  const char* lds_bytes = reinterpret_cast<const char*>(smem);
+
+  const int tid = threadIdx.x;
+  const int lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int group = wave >> 2;
+  const int half = lane >> 5;
+
+  Item item;
+  if (!find_item<kWide, D>(a, blockIdx.x, item)) return;
+  if (item.first && tid == 0 && a.sequence_splits != nullptr)
+    a.sequence_splits[item.b] = int2{item.splits, item.first_slot};
+  const Sequence& seq = item.seq;
+  const int rows = seq.count * a.group;
+  const int q0 = item.block * kRows;
+  const int row0 = q0 + wave * kWaveRows;
+  const int my_row = row0 + (lane & 31);
+  const int last = seq.len - 1;
+
+  // Keys of the block, and this split's tiles. Keys and positions count from its first tile.
+  int kv_end = seq.len;
+  if (a.causal) kv_end = min(kv_end, token_of_row(a, min(q0 + kRows, rows) - 1) + 1 + seq.len - seq.count);
+  const TileRange range = tile_range(item, kv_end > 0 ? (kv_end + kKeys - 1) / kKeys : 0);
+  const int num_tiles = range.end - range.begin;
+  const int key0 = range.begin * kKeys;
+  const int offset = seq.len - seq.count - key0;
+  const int seqlen_k = seq.len - key0;
+  // Tiles this wave sees any key of, and the first whose scores need masking.
+  int my_tiles = num_tiles;
+  int mask_from = seqlen_k / kKeys;
+  if (a.causal) {
+    const int end = token_of_row(a, row0 + kWaveRows - 1) + offset;
+    my_tiles = end < 0 ? 0 : min(num_tiles, end / kKeys + 1);
+    const int x = token_of_row(a, row0) + offset - (kKeys - 1);
+    mask_from = min(mask_from, x < 0 ? 0 : x / kKeys + 1);
+  }
+  if (row0 >= rows) my_tiles = 0;
+  const int last_key = a.causal ? min(seqlen_k - 1, token_of_row(a, my_row) + offset) : seqlen_k - 1;
+
+  u32x4 qf[D / 16];
+  {
+    const bool in = my_row < rows;
+    const int token = token_of_row(a, in ? my_row : 0);
+    const int head = item.hkv * a.group + (in ? my_row : 0) - token * a.group;
+    const uint16_t* src = a.q + (a.c.cu_seqlens ? seq.start * a.q_ss : item.b * a.q_bs) + token * a.q_ss +
+                          head * a.q_hs + 8 * half;
+#pragma unroll
+    for (int ks = 0; ks < D / 16; ++ks) qf[ks] = in ? load16(src + 16 * ks) : u32x4{0, 0, 0, 0};
+  }
+
+  int k_lds[D / 16];
+#pragma unroll
+  for (int ks = 0; ks < D / 16; ++ks) k_lds[ks] = k_lane_offset<D>(ks, lane);
+  // (V offsets are biased by the K ring's size, so that every slot is an immediate.)
+  int v_lds[D / 32][2];
+  int v_bias = kVRingBytes;
+  asm volatile("" : "+v"(v_bias));
+#pragma unroll
+  for (int nb = 0; nb < D / 32; ++nb) {
+    v_lds[nb][0] = v_lane_offset<D>(nb, 0, lane) + v_bias;
+    v_lds[nb][1] = v_lane_offset<D>(nb, 1, lane) + v_bias;
+  }
+
+  // This wave's 16 rows of its group's tensor in every tile: lane l works out where row l % 16 lies, and
+  // piece j of the lane is 16 bytes of row kRowStep j + l / kPerRow.
+  constexpr int kRowStep = 64 / P::kPerRow;
+  constexpr int kPieces = 16 / kRowStep;
+  const int tile_row0 = 16 * (wave & 3);
+  const int piece_row = lane / P::kPerRow;
+  const int piece = lane % P::kPerRow;
+  const bool for_v = group == 1;
+  const RowSpace space = rows_of(a.c, for_v, item.b, item.hkv, P::kElem);
+  const RowSpace scale_space = scales_of(a.c, for_v, item.b, item.hkv);
+  const int ring = for_v ? kVRingBytes : 0;
+  // Rows behind the sequence's last one are not read: it takes their place in K, zeros in V.
+  auto key_of = [&](int t) { return key0 + t * kKeys + tile_row0 + (lane & 15); };
+  int outer = 0;       // slab or block of the row of the next tile to be asked for
+  uint64_t row_at = 0;  // address of that row
+  uint32_t in_scale = 0;
+  auto find = [&](int t) { outer = cache::place(a.c, item.b, min(key_of(t), last)).outer; };
+  auto locate = [&](int t) {
+    const int key = min(key_of(t), last);
+    const cache::Place at{outer, a.c.block_tables == nullptr ? key : cache::row_in_block(a.c, key)};
+    row_at = reinterpret_cast<uint64_t>(space.base) + space.offset(a.c, at);
+    if constexpr (kE4M3) in_scale = static_cast<uint8_t>(scale_space.base[scale_space.offset(a.c, at)]);
+    if (for_v && key_of(t) > last) row_at = reinterpret_cast<uint64_t>(zero_row);
+  };
+  auto address = [&](int j) {
+    const int from = kRowStep * j + piece_row;
+    const uint32_t lo = __shfl(static_cast<int>(row_at), from);
+    const uint32_t hi = __shfl(static_cast<int>(row_at >> 32), from);
+    // (LDS chunk `piece` of a row of 16-bit elements holds the row's chunk piece ^ swz.)
+    const int chunk = kE4M3 ? piece : piece ^ prefill::swz<D>(from);
+    return reinterpret_cast<const char*>(static_cast<uint64_t>(hi) << 32 | lo) + 16 * chunk;
+  };
+  // Tile t's pieces go into its ring slot, codes into the wave's own place.
+  char* codes = reinterpret_cast<char*>(smem) + kCodesAt + wave * 2 * kCodeBytes;
+  const uint32_t lds_wave = __builtin_amdgcn_readfirstlane(
+      kE4M3 ? lds_address(codes) : lds_address(smem) + ring + tile_row0 * 2 * D);
+  auto ask = [&](int t, int slot, int j) {
+    const uint32_t to = kE4M3 ? (t & 1) * kCodeBytes : (static_cast<unsigned>(slot) % kStages) * kSlotBytes;
+    global_load16_to_lds_asm(address(j), lds_wave + to + 1024 * j);
+  };
+  constexpr int kPuts = kE4M3 ? 2 * kPieces : 0;  // 16-byte stores of a tile
+  u32x4 code{};
+  float scale = 0.f;
+  auto put = [&](int t, int slot, int i) {
+    const int j = i / 2;
+    const int row = kRowStep * j + piece_row;
+    uint16_t* tile = reinterpret_cast<uint16_t*>(reinterpret_cast<char*>(smem) + ring +
+                                                 (static_cast<unsigned>(slot) % kStages) * kSlotBytes);
+    const u32x2 lo = cache::values4<Tag>(code[2 * (i % 2)], scale);
+    const u32x2 hi = cache::values4<Tag>(code[2 * (i % 2) + 1], scale);
+    *reinterpret_cast<u32x4*>(tile + tile_offset<D>(tile_row0 + row, 16 * piece + 8 * (i % 2))) =
+        u32x4{lo[0], lo[1], hi[0], hi[1]};
+  };
+  auto take = [&](int t, int j) {  // a piece of tile t's codes, and its row's scale
+    code = *reinterpret_cast<const u32x4*>(codes + (t & 1) * kCodeBytes + 1024 * j + 16 * lane);
+    scale = cache::scale_of(__shfl(static_cast<int>(in_scale), kRowStep * j + piece_row));
+  };
+
+  f32x16 o[D / 32];
+#pragma unroll
+  for (int nb = 0; nb < D / 32; ++nb) o[nb] = f32x16{};
+  f32x16 s0 = f32x16{};
+  f32x16 s1 = f32x16{};
+  u32x4 pf[4] = {};
+  float ref = kNoRef;
+  float l = 0.f;
+  const float sl2 = a.scale_log2;
+
+  // The MFMA phase of a period (prefill_pp.hip): P V of the tile before, K Q^T of this one, 12 P V steps
+  // first, the row max of the new scores between the last 4.
+  constexpr int kPv = 4 * (D / 32);
+  constexpr int kQk = 2 * (D / 16);
+  constexpr int kSteps = kPv + kQk;
+  constexpr int kTail = 4;
+  constexpr int kLeadPv = kPv - kTail;
+  auto step_at = [](auto n_tag, auto full_tag) constexpr {
+    constexpr int n = decltype(n_tag)::value;
+    if constexpr (!decltype(full_tag)::value) {
+      return n;
+    } else {
+      return n < kLeadPv ? n : n < kLeadPv + kQk ? kPv + (n - kLeadPv) : n - kQk;
+    }
+  };
+  auto read_frag = [&](int slot, auto i_tag) -> u32x4 {
+    constexpr int i = decltype(i_tag)::value;
+    if constexpr (i < kPv) {
+      constexpr int kk = i / (D / 32), nb = i % (D / 32);
+      const char* vt = lds_bytes + (static_cast<unsigned>(slot + kStages - 1) % kStages) * kSlotBytes;
+      return v_frag_at(vt + kk * kKeyStepBytes<D>, v_lds[nb][0], v_lds[nb][1]);
+    } else {
+      constexpr int j = i - kPv, ks = j / 2, blk = j % 2;
+      const char* kt = lds_bytes + (static_cast<unsigned>(slot) % kStages) * kSlotBytes;
+      return prefill::lds_load16(kt + blk * kKeyBlockBytes<D>, k_lds[ks]);
+    }
+  };
+  u32x4 pre[kAhead];
+  auto prefetch = [&](int slot) {
+    static_for<0, kAhead>([&](auto i) { pre[decltype(i)::value] = read_frag(slot, i); });
+  };
+  auto prefetch_qk = [&](int slot) {
+    static_for<0, kAhead>([&](auto i) {
+      pre[decltype(i)::value] = read_frag(slot, std::integral_constant<int, kPv + decltype(i)::value>{});
+    });
+  };
+  float tile_mx = kNoRef;
+  float mx_t[10], mx_u[4], mx_w = 0.f;
+  auto max_op = [&](auto k_tag) {
+    constexpr int k = decltype(k_tag)::value;
+    if constexpr (k < 5) {
+      mx_t[k] = max3_f32(s0[3 * k], s0[3 * k + 1], s0[3 * k + 2]);
+    } else if constexpr (k < 10) {
+      mx_t[k] = max3_f32(s1[3 * (k - 5)], s1[3 * (k - 5) + 1], s1[3 * (k - 5) + 2]);
+    } else if constexpr (k < 13) {
+      mx_u[k - 10] = max3_f32(mx_t[3 * (k - 10)], mx_t[3 * (k - 10) + 1], mx_t[3 * (k - 10) + 2]);
+    } else if constexpr (k == 13) {
+      mx_u[3] = max3_f32(mx_t[9], s0[15], s1[15]);
+    } else if constexpr (k == 14) {
+      mx_w = max3_f32(mx_u[0], mx_u[1], mx_u[2]);
+    } else if constexpr (k == 15) {
+      mx_w = max2_f32(mx_w, mx_u[3]);
+    } else if constexpr (k == 16) {
+      mx_w = max_halves(mx_w);
+    } else {
+      tile_mx = mx_w * sl2;
+    }
+  };
+  constexpr int kMaxOps = 18;
+  auto mfma_phase = [&](int slot, auto pv_tag, auto qk_tag, auto&& hook) {
+    constexpr bool kDoPv = decltype(pv_tag)::value;
+    constexpr bool kDoQk = decltype(qk_tag)::value;
+    constexpr bool kFull = kDoPv && kDoQk;
+    constexpr int kFirstLive = kDoPv ? 0 : kPv;
+    constexpr int kEndLive = kDoQk ? kSteps : kPv;
+    u32x4 fr[kSteps];
+    static_for<0, kAhead>([&](auto i) {
+      constexpr int n = kFirstLive + decltype(i)::value;
+      fr[step_at(std::integral_constant<int, n>{}, std::bool_constant<kFull>{})] = pre[decltype(i)::value];
+    });
+    __builtin_amdgcn_s_setprio(1);
+    __builtin_amdgcn_sched_barrier(0);
+    static_for<0, kSteps>([&](auto n_tag) {
+      constexpr int n = decltype(n_tag)::value;
+      constexpr int i = step_at(n_tag, std::bool_constant<kFull>{});
+      if constexpr (n >= kFirstLive && n < kEndLive) {
+        if constexpr (i < kPv) {
+          constexpr int kk = i / (D / 32), nb = i % (D / 32);
+          o[nb] = E::mfma32(fr[i], pf[kk], o[nb]);
+        } else {
+          constexpr int j = i - kPv, ks = j / 2, blk = j % 2;
+          f32x16& acc = blk == 0 ? s0 : s1;
+          acc = E::mfma32(fr[i], qf[ks], ks == 0 ? f32x16{} : acc);
+        }
+      }
+      constexpr int nx = n + kAhead;
+      if constexpr (nx >= kFirstLive + kAhead && nx < kEndLive) {
+        constexpr int ix = step_at(std::integral_constant<int, nx>{}, std::bool_constant<kFull>{});
+        fr[ix] = read_frag(slot, std::integral_constant<int, ix>{});
+      }
+      hook(n_tag);
+      if constexpr (kFull && n >= kLeadPv + kQk) {
+        constexpr int k = n - (kLeadPv + kQk);
+        static_for<k * kMaxOps / kTail, (k + 1) * kMaxOps / kTail>([&](auto op) { max_op(op); });
+      }
+      __builtin_amdgcn_sched_barrier(0);
+    });
+    __builtin_amdgcn_s_setprio(0);
+    if constexpr (kDoQk && !kDoPv) static_for<0, kMaxOps>([&](auto op) { max_op(op); });
+  };
+
+  auto softmax_phase = [&](int t) {
+    float mx = tile_mx;
+    if (t >= mask_from) {
+      asm volatile("" ::: "memory");
+      const int lim = last_key - t * kKeys - 4 * half;
+#pragma unroll
+      for (int j = 0; j < 16; ++j) {
+        const int kj = acc_key(j, 0);
+        s0[j] = kj > lim ? -INFINITY : s0[j];
+        s1[j] = kj + 32 > lim ? -INFINITY : s1[j];
+        __builtin_amdgcn_sched_barrier(0);  // (one compare and one select at a time: prefill_pp.hip)
+      }
+      mx = max_halves(max_of(s0, s1)) * sl2;
+    }
+    if (wave_any(mx > ref + kMoveSlack)) {
+      asm volatile("" ::: "memory");
+      const float moved = max2_f32(ref, mx);
+      const float alpha = exp2_fast(ref - moved);  // 0 for a row's first key
+      ref = moved;
+#pragma unroll
+      for (int nb = 0; nb < D / 32; ++nb) o[nb] *= alpha;
+      l *= alpha;
+    }
+    f32x16 p0, p1;
+#pragma unroll
+    for (int j = 0; j < 16; ++j) {
+      p0[j] = exp2_fast(fmaf(s0[j], sl2, -ref));
+      p1[j] = exp2_fast(fmaf(s1[j], sl2, -ref));
+    }
+    float r0 = p0[0];
+    float r1 = p1[0];
+#pragma unroll
+    for (int j = 1; j < 16; ++j) {
+      r0 += p0[j];
+      r1 += p1[j];
+    }
+    pf[0] = p_frag<Tag, 0>(p0);
+    pf[1] = p_frag<Tag, 1>(p0);
+    pf[2] = p_frag<Tag, 0>(p1);
+    pf[3] = p_frag<Tag, 1>(p1);
+    l += r0 + r1;
+  };
+
+  using kFirstT = std::integral_constant<int, 0>;
+  using kFullT = std::integral_constant<int, 1>;
+  using kLastT = std::integral_constant<int, 2>;
+  using kLoadsT = std::integral_constant<int, 3>;
+  auto run = [&](auto group_tag) {
+    constexpr int kGroup = decltype(group_tag)::value;
+    auto period = [&](int m, int slot, auto mode_tag) {
+      constexpr int kMode = decltype(mode_tag)::value;
+      constexpr bool kDoPv = kMode == kFullT::value || kMode == kLastT::value;
+      constexpr bool kDoQk = kMode == kFirstT::value || kMode == kFullT::value;
+      auto hook = [&](auto i_tag) {
+        constexpr int i = decltype(i_tag)::value;
+        // (Tile m + 1's loads into LDS, asked for a period ago, have landed; the barrier publishes them.)
+        if constexpr (i == 0) prefill::pp::wait_vmcnt<0>();
+        if constexpr (i % 6 == 0 && i / 3 < kPuts) take(m + 1, i / 6);
+        if constexpr (i % 3 == 2 && i / 3 < kPuts) put(m + 1, slot + 1, i / 3);
+        constexpr int kAskFrom = 3 * kPuts + 1;
+        if constexpr (i == kAskFrom) locate(m + 2);
+        constexpr int k = i - kAskFrom - 2;
+        if constexpr (k >= 0 && k % 3 == 0 && k / 3 < kPieces) ask(m + 2, slot + 2, k / 3);
+        constexpr int kAfter = kAskFrom + 2 + 3 * kPieces;
+        if constexpr (i == kAfter) find(m + 3);
+        static_assert(kAfter < kSteps, "the tile's moves fit the phase");
+      };
+      auto mfma = [&]() {
+        if constexpr (kMode == kLoadsT::value) {
+          static_for<0, kSteps>([&](auto i) { hook(i); });
+        } else {
+          mfma_phase(slot, std::bool_constant<kDoPv>{}, std::bool_constant<kDoQk>{}, hook);
+        }
+      };
+      if constexpr (kGroup == 0) {
+        if constexpr (kMode == kFirstT::value) prefetch_qk(slot);
+        mfma();
+        if constexpr (kDoQk) {
+          prefetch(slot + 1);
+          softmax_phase(m);
+        }
+      } else {
+        if constexpr (kMode == kFirstT::value) prefetch_qk(slot);
+        if constexpr (kDoPv) {
+          prefetch(slot);
+          softmax_phase(m - 1);
+        }
+        mfma();
+      }
+      phase_barrier();
+    };
+    int m = 0;
+    if (my_tiles > 0) {
+      period(0, 0, kFirstT{});
+      for (m = 1; m < my_tiles;) {
+        bool done = false;
+        static_for<0, kStages>([&](auto j) {
+          if (done) return;
+          period(m, (1 + decltype(j)::value) % kStages, kFullT{});
+          done = ++m == my_tiles;
+        });
+      }
+      period(m, m % kStages, kLastT{});
+      ++m;
+    }
+    for (; m <= num_tiles; ++m) period(m, m % kStages, kLoadsT{});
+  };
+  if (num_tiles > 0) {
+    find(0);
+    locate(0);
+    static_for<0, kPieces>([&](auto j) { ask(0, 0, decltype(j)::value); });
+    find(1);
+    prefill::pp::wait_vmcnt<0>();
+    static_for<0, kPuts>([&](auto i) {
+      if constexpr (decltype(i)::value % 2 == 0) take(0, decltype(i)::value / 2);
+      put(0, 0, decltype(i)::value);
+    });
+    locate(1);
+    static_for<0, kPieces>([&](auto j) { ask(1, 1, decltype(j)::value); });
+    find(2);
+    phase_barrier();
+    if (group == 0) {
+      run(std::integral_constant<int, 0>{});
+    } else {
+      run(std::integral_constant<int, 1>{});
+    }
+  }
+
+  prefill::pp::wait_vmcnt<0>();  // (the loads of tiles past the end have landed before LDS is used again)
+  phase_barrier();
+  // Rows leave whole: each wave stages its 32 in its own part of the (free) rings, padded by 16 bytes.
+  const float lt = sum_halves(l);
+  const bool partial = item.splits > 1;
+  constexpr int kStageRow = 4 * D + 16;
+  static_assert(kWaves * 16 * kStageRow <= static_cast<int>(sizeof(smem)), "16 rows of each wave fit");
+  char* stage = reinterpret_cast<char*>(smem) + wave * 16 * kStageRow;
+  const float inv = inverse(lt);
+  if (partial) {
+    // (In two halves of 16 rows.)
+    float* po = a.partial_o + (a.wide_partials + static_cast<int64_t>(item.slot) * kRows + wave * kWaveRows) * D;
+#pragma unroll
+    for (int part = 0; part < 2; ++part) {
+      if (((lane >> 4) & 1) == part) {
+        char* w = stage + (lane & 15) * kStageRow + 16 * half;
+#pragma unroll
+        for (int nb = 0; nb < D / 32; ++nb) {
+#pragma unroll
+          for (int g = 0; g < 4; ++g)
+            *reinterpret_cast<f32x4*>(w + 32 * (4 * nb + g)) =
+                f32x4{o[nb][4 * g], o[nb][4 * g + 1], o[nb][4 * g + 2], o[nb][4 * g + 3]};
+        }
+      }
+      const int r2 = lane / 32;  // two rows per store instruction
+      for (int j = 0; j < 8; ++j) {
+        const int r = 16 * part + 2 * j + r2;
+        const f32x4 x = *reinterpret_cast<const f32x4*>(stage + (2 * j + r2) * kStageRow + 16 * (lane & 31));
+        if (row0 + r < rows) *reinterpret_cast<f32x4*>(po + r * D + 4 * (lane & 31)) = x;
+      }
+    }
+    if (my_row < rows && half == 0)
+      a.partial_ml[a.wide_partials + static_cast<int64_t>(item.slot) * kRows + my_row - q0] = point_and_sum(ref, lt);
+    return;
+  }
+  constexpr int kOutRow = 2 * D + 16;
+  stage = reinterpret_cast<char*>(smem) + wave * kWaveRows * kOutRow;
+  {
+    char* w = stage + (lane & 31) * kOutRow + 8 * half;
+#pragma unroll
+    for (int nb = 0; nb < D / 32; ++nb) {
+#pragma unroll
+      for (int g = 0; g < 4; ++g)
+        *reinterpret_cast<u32x2*>(w + 16 * (4 * nb + g)) =
+            u32x2{E::pack2(o[nb][4 * g] * inv, o[nb][4 * g + 1] * inv),
+                  E::pack2(o[nb][4 * g + 2] * inv, o[nb][4 * g + 3] * inv)};
+    }
+  }
+  uint16_t* out = a.o + (a.c.cu_seqlens ? seq.start * a.o_ss : item.b * a.o_bs) + 8 * (lane & 15);
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    const int r = 4 * j + (lane >> 4);
+    const u32x4 x = *reinterpret_cast<const u32x4*>(stage + r * kOutRow + 16 * (lane & 15));
+    if (row0 + r < rows) {
+      const int token = token_of_row(a, row0 + r);
+      const int head = item.hkv * a.group + row0 + r - token * a.group;
+      *reinterpret_cast<u32x4*>(out + token * a.o_ss + head * a.o_hs) = x;
+    }
+  }
+  if (my_row < rows && half == 0) {
+    const int token = token_of_row(a, my_row);
+    a.lse[(static_cast<int64_t>(seq.start) + token) * a.heads + item.hkv * a.group + my_row - token * a.group] =
+        log_sum(ref, lt);
+  }
+}
+
+template <typename Tag>
+hipError_t launch_typed(const CachedAttnArgs& args, int64_t workgroups, bool e4m3, hipStream_t stream) {
+  const dim3 grid(static_cast<uint32_t>(workgroups));
+  if (e4m3) {
+    hipLaunchKernelGGL((cached_pp_kernel<Tag, true>), grid, dim3(kThreads), 0, stream, args);
+  } else {
+    hipLaunchKernelGGL((cached_pp_kernel<Tag, false>), grid, dim3(kThreads), 0, stream, args);
+  }
+  return hipGetLastError();
+}
+
+}  // namespace
+}  // namespace cached
+
+hipError_t launch_cached_pp(const CachedAttnArgs& args, int64_t workgroups, DType dtype, bool e4m3,
+                            hipStream_t stream) {
+  using namespace cached;
+  return dtype == DType::bf16 ? launch_typed<bf16_tag>(args, workgroups, e4m3, stream)
+                              : launch_typed<f16_tag>(args, workgroups, e4m3, stream);
+}
+
+}  // namespace fl

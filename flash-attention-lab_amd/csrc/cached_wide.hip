@@ -29,7 +29,7 @@ using prefill::v_lane_offset;
 constexpr int kWaves = 4;
 constexpr int kThreads = 64 * kWaves;
 constexpr int kWaveRows = 32;
-constexpr int kRows = kWideRows;
+constexpr int kRows = block_rows(kWide, 64);
 static_assert(kRows == kWaves * kWaveRows, "a wave per 32 rows");
 
 // A piece into a tile in LDS, as Tag's elements.
@@ -52,7 +52,7 @@ __device__ __forceinline__ void wide_item(const CachedAttnArgs& a, const Item& i
   using E = Elem<Tag>;
   constexpr int kTile = kTileElems<D>;
   // Two slots of K tiles, of V tiles, of rows' offsets (K, V) and of scales (K, V).
-  int64_t* offsets = reinterpret_cast<int64_t*>(smem + 4 * kTile);
+  uint64_t* offsets = reinterpret_cast<uint64_t*>(smem + 4 * kTile);
   float* scales = reinterpret_cast<float*>(offsets + 4 * kKeys);
   auto k_lds = [&](int slot) { return smem + slot * kTile; };
   auto v_lds = [&](int slot) { return smem + (2 + slot) * kTile; };
@@ -106,13 +106,12 @@ __device__ __forceinline__ void wide_item(const CachedAttnArgs& a, const Item& i
   const int load_row = tid / P::kPerRow;
   const int load_col = tid % P::kPerRow * P::kElems;
   const int last = seq.len - 1;  // rows behind it are not read: it takes their place in K, zeros in V
-  const char* kp = a.c.k + (item.hkv * a.c.k_hs + load_col) * P::kElem;
-  const char* vp = a.c.v + (item.hkv * a.c.v_hs + load_col) * P::kElem;
   const bool for_v = wave & 1;
   const bool for_scale = wave >> 1;
-  const uint8_t* my_scales = for_v ? a.c.v_scales + item.hkv * a.c.vs_hs : a.c.k_scales + item.hkv * a.c.ks_hs;
-  RowSpace space{(for_v ? a.c.v_bs : a.c.k_bs) * P::kElem, (for_v ? a.c.v_ss : a.c.k_ss) * P::kElem};
-  if (kE4M3 && for_scale) space = for_v ? RowSpace{a.c.vs_bs, a.c.vs_ss} : RowSpace{a.c.ks_bs, a.c.ks_ss};
+  const RowSpace space = kE4M3 && for_scale ? scales_of(a.c, for_v, item.b, item.hkv)
+                                            : rows_of(a.c, for_v, item.b, item.hkv, P::kElem);
+  const char* kp = rows_of(a.c, false, item.b, item.hkv, P::kElem).base + load_col * P::kElem;
+  const char* vp = rows_of(a.c, true, item.b, item.hkv, P::kElem).base + load_col * P::kElem;
   struct Pieces {
     u32x4 k[kPieces], v[kPieces];
   };
@@ -122,7 +121,7 @@ __device__ __forceinline__ void wide_item(const CachedAttnArgs& a, const Item& i
     if (!for_scale) {
       offsets[((tile & 1) * 2 + wave) * kKeys + lane] = space.offset(a.c, at);
     } else if constexpr (kE4M3) {
-      byte = my_scales[space.offset(a.c, at)];
+      byte = static_cast<uint8_t>(space.base[space.offset(a.c, at)]);
     }
   };
   auto put_scales = [&](int tile, uint32_t byte) {
@@ -131,7 +130,7 @@ __device__ __forceinline__ void wide_item(const CachedAttnArgs& a, const Item& i
     }
   };
   auto load = [&](int tile, Pieces& r) {
-    const int64_t* at = offsets + (tile & 1) * 2 * kKeys + load_row;
+    const uint64_t* at = offsets + (tile & 1) * 2 * kKeys + load_row;
 #pragma unroll
     for (int j = 0; j < kPieces; ++j) {
       r.k[j] = load16(kp + at[j * kRowStep]);
@@ -286,7 +285,7 @@ __global__ void __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2
     cached_wide_kernel(const CachedAttnArgs a) {
   __shared__ __attribute__((aligned(16))) uint16_t smem[4 * kTileElems<D> + 4 * kKeys * (8 + 4) / 2];
   Item item;
-  if (!find_item<kWide>(a, blockIdx.x, item)) return;
+  if (!find_item<kWide, D>(a, blockIdx.x, item)) return;
   if (item.first && threadIdx.x == 0 && a.sequence_splits != nullptr)
     a.sequence_splits[item.b] = int2{item.splits, item.first_slot};
   wide_item<Tag, D, kE4M3>(a, item, smem);
@@ -309,12 +308,9 @@ hipError_t launch_typed(const CachedAttnArgs& args, int64_t workgroups, bool e4m
 hipError_t launch_cached_wide(const CachedAttnArgs& args, int64_t workgroups, DType dtype, bool e4m3, int head_dim,
                               hipStream_t stream) {
   using namespace cached;
-  if (dtype == DType::bf16) {
-    return head_dim == 64 ? launch_typed<bf16_tag, 64>(args, workgroups, e4m3, stream)
-                          : launch_typed<bf16_tag, 128>(args, workgroups, e4m3, stream);
-  }
-  return head_dim == 64 ? launch_typed<f16_tag, 64>(args, workgroups, e4m3, stream)
-                        : launch_typed<f16_tag, 128>(args, workgroups, e4m3, stream);
+  if (head_dim == 128) return launch_cached_pp(args, workgroups, dtype, e4m3, stream);
+  return dtype == DType::bf16 ? launch_typed<bf16_tag, 64>(args, workgroups, e4m3, stream)
+                              : launch_typed<f16_tag, 64>(args, workgroups, e4m3, stream);
 }
 
 }  // namespace fl

@@ -148,6 +148,11 @@ __device__ __forceinline__ void buffer_load16_to_lds_asm(u32x4s words, uint32_t 
                : "v"(offset), "s"(m0), "s"(w)
                : "memory", "m0");
 }
+// The same from an address per lane: lane l's 16 bytes at p go to LDS at lds_addr + 16 l.
+__device__ __forceinline__ void global_load16_to_lds_asm(const void* p, uint32_t lds_addr) {
+  const uint32_t m0 = static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<int>(lds_addr)));
+  asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" : : "v"(p), "s"(m0) : "memory", "m0");
+}
 // 32-bit LDS address of a __shared__ object.
 __device__ __forceinline__ uint32_t lds_address(const void* p) {
   typedef __attribute__((address_space(3))) const void lds_cvoid;
