@@ -940,7 +940,7 @@ int fl_cached_attention(const fl_cached_attn_params* p, int32_t cu_count, fl_str
     if (!aligned(p->workspace, 16)) return fail(FL_ERR_INVALID, "attention workspace must be 16-byte aligned");
     a.partial_o = p->workspace;
     a.partial_ml = reinterpret_cast<fl::f32pair*>(a.partial_o + plan.partial_rows * c.head_dim);
-    a.sequence_splits = reinterpret_cast<int2*>(a.partial_ml + plan.partial_rows);
+    a.merge_blocks = reinterpret_cast<fl::MergeBlock*>(a.partial_ml + plan.partial_rows);
   }
   const hipError_t err = fl::launch_cached_attn(a, plan, decode_dtype(p->dtype), c.dtype == FL_DTYPE_E4M3, c.head_dim,
                                                 static_cast<hipStream_t>(stream));

@@ -17,8 +17,10 @@ namespace cached {
 enum Kind { kNarrow, kWide };
 constexpr int kNarrowRows = 48;  // most rows of a narrow sequence
 constexpr int kKeys = 64;        // keys of a tile: splits are whole tiles
-constexpr int kStartTiles = 4;   // tiles that starting and ending an item costs as much as
-constexpr int kMaxRounds = 3;
+// Tiles that starting and ending an item costs as much as.
+__host__ __device__ __forceinline__ constexpr int start_tiles(Kind kind) { return kind == kNarrow ? 4 : 6; }
+// From so many rounds of blocks on they run whole, as they come, the longest first.
+constexpr int kWholeRounds = 6;
 // Rows of a block.
 __host__ __device__ __forceinline__ constexpr int block_rows(Kind kind, int head_dim) {
   return kind == kNarrow ? kNarrowRows : head_dim == 128 ? 256 : 128;
@@ -46,109 +48,124 @@ __device__ __forceinline__ float wave_sum(float x) {
   return x;
 }
 
-// A workgroup's item: one split of one block of rows of one KV head of one sequence.
+// Sums over the sequences of a batch: lane l holds sequence 64 i + l of chunk i; chunks behind the first are
+// read again in every pass.
+struct Batch {
+  const CachedAttnArgs& a;
+  Sequence first;
+  __device__ __forceinline__ explicit Batch(const CachedAttnArgs& args) : a(args), first(at(__lane_id())) {}
+  __device__ __forceinline__ Sequence at(int b) const {
+    Sequence s{0, 0, 0};
+    if (b < a.c.batch) s = cache::sequence(a.c, b);
+    return s;
+  }
+  __device__ __forceinline__ Sequence lane_of(int base) const { return base == 0 ? first : at(base + __lane_id()); }
+  template <typename F>
+  __device__ __forceinline__ auto sum(F f) const {
+    auto total = f(first);
+    for (int base = 64; base < a.c.batch; base += 64) total += f(at(base + __lane_id()));
+    return wave_sum(total);
+  }
+  // Sequences that overlap (cu_seqlens does not ascend) could have more items than the grid and the
+  // workspace are made for: no item is run then.
+  __device__ __forceinline__ bool sound() const {
+    return a.c.cu_seqlens == nullptr ||
+           sum([](const Sequence& s) { return static_cast<float>(s.count); }) <= 1.001f * a.c.tokens;
+  }
+};
+
+// Blocks of rows of a sequence (none, if it is of the other kind), and its key tiles.
+template <Kind kKind, int D>
+__device__ __forceinline__ int blocks_of(const CachedAttnArgs& a, const Sequence& s) {
+  const int rows = s.count * a.group;
+  const bool mine = (rows <= kNarrowRows) == (kKind == kNarrow);
+  return mine ? (rows + block_rows(kKind, D) - 1) / block_rows(kKind, D) : 0;
+}
+__device__ __forceinline__ int tiles_of(const Sequence& s) { return (s.len + kKeys - 1) / kKeys; }
+// Key tiles that block i of a sequence sees any key of.
+template <Kind kKind, int D>
+__device__ __forceinline__ int block_tiles(const CachedAttnArgs& a, const Sequence& s, int i) {
+  int end = s.len;
+  if (a.causal) {
+    const int rows = min((i + 1) * block_rows(kKind, D), s.count * a.group);
+    end = max(min(end, token_of_row(a, max(rows - 1, 0)) + 1 + s.len - s.count), 0);
+  }
+  return (end + kKeys - 1) / kKeys;
+}
+
+// A workgroup's item: key tiles begin .. end - 1 of one block of rows of one KV head of one sequence. Not all
+// of the block's: what it leaves are partials, in slot `slot`.
 struct Item {
-  int b, hkv, block, split, splits;
-  int slot;        // of its partials, splits > 1
-  int first_slot;  // of the sequence
-  bool first;      // the sequence's first item
+  int b, hkv, block, begin, end;
+  bool partial;
+  int slot;
   Sequence seq;
 };
 
-// Blocks of rows and key tiles of a sequence; no blocks, if it is of the other kind.
-struct Load {
-  int blocks, tiles;
-};
-template <Kind kKind, int D>
-__device__ __forceinline__ Load load_of(const CachedAttnArgs& a, const Sequence& s) {
-  const int rows = s.count * a.group;
-  const bool mine = (rows <= kNarrowRows) == (kKind == kNarrow);
-  return Load{mine ? (rows + block_rows(kKind, D) - 1) / block_rows(kKind, D) : 0, (s.len + kKeys - 1) / kKeys};
+// The same values, for the compiler to keep in scalar registers.
+__device__ __forceinline__ Item uniform(const Item& i) {
+  auto u = [](int x) { return __builtin_amdgcn_readfirstlane(x); };
+  return Item{u(i.b), u(i.hkv), u(i.block), u(i.begin), u(i.end), u(i.partial) != 0, u(i.slot),
+              Sequence{u(i.seq.start), u(i.seq.count), u(i.seq.len)}};
 }
 
-// The items of a kernel, over the sequences of its kind: sequence b has blocks_b splits_b H_kv of them, with splits_b = ceil(tiles_b / share). a.slots
-// workgroups run at once, so items of up to `share` tiles that fill r rounds of slots end after about
-// r (share + what starting an item costs): share and r are chosen for the least of that, with the least
-// share for which no more than r slots items result. Within a chunk of 64 sequences longer items come
-// first where there is more than one round, so that the last ones to start are short. Lane l holds sequence
-// 64 i + l of chunk i; chunks behind the first are read again in every pass.
+// What the merge needs of a block whose first partial the workgroup leaves (cached_attn.hip): in the workgroup's own
+// place of the list.
+__device__ __forceinline__ void leave(const CachedAttnArgs& a, const Item& item, int splits) {
+  if (threadIdx.x == 0 && static_cast<int>(blockIdx.x) < a.merges)
+    a.merge_blocks[blockIdx.x] = MergeBlock{splits, item.slot, item.b, item.hkv, item.block, item.seq.start, item.seq.count, 0};
+}
+
+// Items of equal shares: sequence b has blocks_b splits_b H_kv of them, with splits_b = ceil(tiles_b / share).
+// The least share for which no more than `slots` items result (which run at once), 0 if there are more blocks.
 template <Kind kKind, int D>
-__device__ __forceinline__ bool find_item(const CachedAttnArgs& a, int id, Item& item) {
-  const int lane = __lane_id();
-  const int batch = a.c.batch;
-  auto sequence_at = [&](int b) {
-    Sequence s{0, 0, 0};
-    if (b < batch) s = cache::sequence(a.c, b);
-    return s;
+__device__ __forceinline__ int even_share(const CachedAttnArgs& a, const Batch& batch, int blocks, int slots) {
+  if (blocks > slots) return 0;
+  auto items = [&](int t) {
+    return a.c.heads_kv * batch.sum([&](const Sequence& s) {
+      return blocks_of<kKind, D>(a, s) * max((tiles_of(s) + t - 1) / t, 1);
+    });
   };
-  const Sequence first = sequence_at(lane);
-  const Load first_load = load_of<kKind, D>(a, first);
-  // f(blocks, tiles) summed over all sequences.
-  auto sum = [&](auto f) {
-    auto total = f(first_load);
-    for (int base = 64; base < batch; base += 64) total += f(load_of<kKind, D>(a, sequence_at(base + lane)));
-    return wave_sum(total);
-  };
-  // Sequences that overlap (cu_seqlens does not ascend) could have more items than the grid and the
-  // workspace are made for: no item is run then.
-  if (a.c.cu_seqlens != nullptr) {
-    float tokens = first.count;
-    for (int base = 64; base < batch; base += 64) tokens += sequence_at(base + lane).count;
-    if (wave_sum(tokens) > 1.001f * a.c.tokens) return false;
-  }
-  int share = 1 << 30;  // tiles of a split
-  int rounds = 2;       // (more than one)
-  if (a.num_splits == 0 && a.slots > 0) {
-    const int blocks = a.c.heads_kv * sum([](const Load& l) { return l.blocks; });
-    const float work = a.c.heads_kv * sum([](const Load& l) { return float(l.blocks) * float(l.tiles); });
-    auto items = [&](int t) {
-      return a.c.heads_kv * sum([t](const Load& l) { return l.blocks * max((l.tiles + t - 1) / t, 1); });
-    };
-    float least = INFINITY;
-    for (int r = 1; r <= a.max_rounds; ++r) {
-      const int slots = r * a.slots;
-      if (blocks > slots) continue;
-      // sum of ceil(x / t) is at most work / t + blocks.
-      int low = max(a.min_tiles, static_cast<int>(work / slots));
-      int high = blocks < slots ? max(low, static_cast<int>(work / (slots - blocks) * 1.001f) + 1) : 1 << 28;
-      while (low < high) {
-        const int mid = low + (high - low) / 2;
-        if (items(mid) <= slots) {
-          high = mid;
-        } else {
-          low = mid + 1;
-        }
-      }
-      if (items(low) > slots) continue;
-      const float time = r * static_cast<float>(low + kStartTiles);
-      if (time < least) {
-        least = time;
-        share = low;
-        rounds = r;
-      }
-      // (More rounds can't gain on one that is close to an even share.)
-      if (low <= work / a.slots + kStartTiles) break;
+  const float work = a.c.heads_kv * batch.sum([&](const Sequence& s) {
+    return static_cast<float>(blocks_of<kKind, D>(a, s)) * static_cast<float>(tiles_of(s));
+  });
+  // sum of ceil(x / t) is at most work / t + blocks.
+  int low = max(a.min_tiles, static_cast<int>(work / slots));
+  int high = blocks < slots ? max(low, static_cast<int>(work / (slots - blocks) * 1.001f) + 1) : 1 << 28;
+  while (low < high) {
+    const int mid = low + (high - low) / 2;
+    if (items(mid) <= slots) {
+      high = mid;
+    } else {
+      low = mid + 1;
     }
   }
-  auto splits_of = [&](const Load& l) {
-    return a.num_splits > 0 ? a.num_splits : max((l.tiles + share - 1) / share, 1);
-  };
+  return items(low) <= slots ? low : 0;
+}
+
+// Item `id` of the equal shares (or of a.num_splits splits of every block; share 0: one each). Within a chunk
+// of 64 sequences longer items come first with `sorted`, and within a sequence the blocks that see more keys.
+// The partials of a block lie in consecutive slots.
+template <Kind kKind, int D>
+__device__ __forceinline__ bool find_item(const CachedAttnArgs& a, const Batch& batch, int id, int share, bool sorted,
+                                          Item& item) {
   int before = 0;       // items of earlier chunks
   int before_slot = 0;  // slots of earlier chunks
-  for (int base = 0; base < batch; base += 64) {
-    const Sequence s = base == 0 ? first : sequence_at(base + lane);
-    const Load l = load_of<kKind, D>(a, s);
-    const int splits = splits_of(l);
-    const int items = l.blocks * splits * a.c.heads_kv;
+  for (int base = 0; base < a.c.batch; base += 64) {
+    const int lane = __lane_id();
+    const Sequence s = batch.lane_of(base);
+    const int tiles = tiles_of(s);
+    const int splits = a.num_splits > 0 ? a.num_splits : share > 0 ? max((tiles + share - 1) / share, 1) : 1;
+    const int items = blocks_of<kKind, D>(a, s) * splits * a.c.heads_kv;
     const int slots = splits > 1 ? items : 0;
     const int all = wave_inclusive_sum(items);
     const int all_slots = wave_inclusive_sum(slots);
     int from = all - items;  // items and slots of the chunk before the lane's
     int from_slot = all_slots - slots;
-    if (rounds > 1) {
-      const int length = l.tiles / splits;
+    if (sorted) {
+      const int length = tiles / splits;
       from = from_slot = 0;
-      const int here = min(batch - base, 64);
+      const int here = min(a.c.batch - base, 64);
       for (int j = 0; j < here; ++j) {
         const int other = __builtin_amdgcn_readlane(length, j);
         const bool ahead = other > length || (other == length && j < lane);
@@ -163,17 +180,20 @@ __device__ __forceinline__ bool find_item(const CachedAttnArgs& a, int id, Item&
       auto of_owner = [&](int x) { return __builtin_amdgcn_readlane(x, owner); };
       item.b = base + owner;
       item.seq = Sequence{of_owner(s.start), of_owner(s.count), of_owner(s.len)};
-      item.splits = of_owner(splits);
+      const int n = of_owner(splits);
       const int at = of_owner(local);
-      const int units = a.c.heads_kv * item.splits;  // items of a block
-      const int turn = at / units;                   // blocks with more keys first
+      const int units = a.c.heads_kv * n;  // items of a block
+      const int turn = at / units;
       const int unit = at - turn * units;
-      item.hkv = unit / item.splits;
-      item.split = unit - item.hkv * item.splits;
-      item.block = of_owner(l.blocks) - 1 - turn;
-      item.first_slot = before_slot + of_owner(from_slot);
-      item.slot = item.first_slot + at;
-      item.first = at == 0;
+      item.hkv = unit / n;
+      const int split = unit - item.hkv * n;
+      item.block = of_owner(items) / units - 1 - turn;
+      const int all_tiles = block_tiles<kKind, D>(a, item.seq, item.block);
+      item.begin = static_cast<int>(static_cast<int64_t>(all_tiles) * split / n);
+      item.end = static_cast<int>(static_cast<int64_t>(all_tiles) * (split + 1) / n);
+      item.partial = n > 1;
+      item.slot = before_slot + of_owner(from_slot) + at;
+      if (item.partial && split == 0) leave(a, item, n);
       return true;
     }
     before += __builtin_amdgcn_readlane(all, 63);
@@ -181,6 +201,128 @@ __device__ __forceinline__ bool find_item(const CachedAttnArgs& a, int id, Item&
   }
   return false;
 }
+
+// The line: the blocks of all sequences of a kind one after the other, a block as long as its tiles and what
+// starting it costs, cut into equal chunks for the workgroups: all end together, and no more than two
+// partials a workgroup result. A sequence's blocks go in pairs from its two ends, i and n - 1 - i, the one that
+// sees more keys first: under a causal mask a pair's tiles are about the same for all i (the lighter block
+// counts as what is missing to that), so that a position's block follows without a search.
+template <Kind kKind, int D>
+struct SequenceLine {
+  int n, pairs, pair_tiles, pair_length, length;  // blocks, pairs, tiles and length of a pair, length of a KV head's line
+  static constexpr int kStart = start_tiles(kKind);
+  __device__ __forceinline__ SequenceLine(const CachedAttnArgs& a, const Sequence& s) {
+    n = blocks_of<kKind, D>(a, s);
+    pairs = n / 2;
+    pair_tiles = block_tiles<kKind, D>(a, s, n - 1) + block_tiles<kKind, D>(a, s, 0);
+    pair_length = pair_tiles + 2 * kStart;
+    length = pairs * pair_length + (n & 1 ? block_tiles<kKind, D>(a, s, pairs) + kStart : 0);
+  }
+  // A block's place: where it starts, and the tiles that it counts as.
+  struct Span {
+    int block, start, tiles;
+  };
+  __device__ __forceinline__ Span span_of(const CachedAttnArgs& a, const Sequence& s, int block) const {
+    const bool light = block < pairs;
+    const int heavy = block_tiles<kKind, D>(a, s, light ? n - 1 - block : block);
+    if (light) return Span{block, block * pair_length + heavy + kStart, pair_tiles - heavy};
+    return Span{block, (n - 1 - block) * pair_length, heavy};
+  }
+  __device__ __forceinline__ Span span_at(const CachedAttnArgs& a, const Sequence& s, int position) const {
+    const int pair = min(position / pair_length, pairs);
+    const Span heavy = span_of(a, s, n - 1 - pair);
+    return pair < pairs && position >= heavy.start + heavy.tiles + kStart ? span_of(a, s, pair) : heavy;
+  }
+};
+
+// The segments that a workgroup runs, of one schedule or the other, which every workgroup derives from the
+// lengths alike:
+//  * equal shares, one item a workgroup, where the blocks are few and divide evenly enough;
+//  * a chunk of the line;
+//  * whole blocks as they come, where there are many rounds of them (or no workspace).
+template <Kind kKind, int D>
+struct Segments {
+  int mode, share, chunk, position, end;
+  enum { kShares, kLine, kWhole, kDone };
+  __device__ __forceinline__ explicit Segments(const CachedAttnArgs& a)
+      : mode(kWhole), share(0), chunk(0), position(0), end(0) {
+    // (No block whose partials start here, until there is one.)
+    if (threadIdx.x == 0 && static_cast<int>(blockIdx.x) < a.merges) a.merge_blocks[blockIdx.x].splits = 0;
+    const Batch batch(a);
+    const int blocks = a.c.heads_kv * batch.sum([&](const Sequence& s) { return blocks_of<kKind, D>(a, s); });
+    if (blocks == 0 || !batch.sound()) {
+      mode = kDone;
+      return;
+    }
+    if (a.num_splits > 0 || a.slots == 0 || blocks > kWholeRounds * a.slots) return;
+    const int total = a.line ? a.c.heads_kv * batch.sum([&](const Sequence& s) {
+      return SequenceLine<kKind, D>(a, s).length;
+    }) : 0;
+    chunk = max((total + a.slots - 1) / a.slots, a.min_tiles + start_tiles(kKind));
+    share = even_share<kKind, D>(a, batch, blocks, a.slots);
+    // (A chunk's workgroup starts one more segment than its length counts, and leaves two partials: the line has
+    // to gain more than that.)
+    if (share > 0 && (!a.line || share <= chunk + 2 * start_tiles(kKind))) {
+      mode = kShares;
+    } else if (a.line) {
+      mode = kLine;
+      position = min(static_cast<int>(blockIdx.x) * chunk, total);  // (chunk <= total / slots + a few)
+      end = min(position + chunk, total);
+      position = __builtin_amdgcn_readfirstlane(position);
+      end = __builtin_amdgcn_readfirstlane(end);
+      chunk = __builtin_amdgcn_readfirstlane(chunk);
+    }
+  }
+  __device__ __forceinline__ bool next(const CachedAttnArgs& a, Item& item) {
+    if (mode == kDone || (mode == kLine && position >= end)) return false;
+    const Batch batch(a);  // (read again for each segment: kept, it would take registers from the item)
+    if (mode != kLine) {
+      const bool found = find_item<kKind, D>(a, batch, blockIdx.x, share, mode == kWhole, item);
+      mode = kDone;
+      return found;
+    }
+    while (position < end) {
+      int before = 0;
+      for (int base = 0; base < a.c.batch; base += 64) {
+        const Sequence s = batch.lane_of(base);
+        const int length = SequenceLine<kKind, D>(a, s).length * a.c.heads_kv;
+        const int through = before + wave_inclusive_sum(length);
+        const uint64_t mask = __builtin_amdgcn_ballot_w64(position < through);
+        if (mask == 0) {
+          before = __builtin_amdgcn_readlane(through, 63);
+          continue;
+        }
+        const int owner = __builtin_ctzll(mask);
+        auto of_owner = [&](int x) { return __builtin_amdgcn_readlane(x, owner); };
+        item.b = base + owner;
+        item.seq = Sequence{of_owner(s.start), of_owner(s.count), of_owner(s.len)};
+        const int origin = of_owner(through) - of_owner(length);  // of the sequence
+        const SequenceLine<kKind, D> line(a, item.seq);
+        item.hkv = (position - origin) / line.length;
+        const int start = origin + item.hkv * line.length;  // of the KV head
+        const auto span = line.span_at(a, item.seq, position - start);
+        item.block = span.block;
+        const int from = position - start - span.start;
+        const int to = min(from + end - position, span.tiles);
+        const int tiles = block_tiles<kKind, D>(a, item.seq, span.block);
+        // (The last segment takes what the block has; a lighter block can count as a tile more or less.)
+        item.begin = min(from, tiles);
+        item.end = to == span.tiles ? tiles : min(to, tiles);
+        item.partial = from > 0 || to < span.tiles;
+        item.slot = 2 * static_cast<int>(blockIdx.x) + (from == 0 ? 1 : 0);
+        const bool any = from == 0 || from < span.tiles;  // (not only what a start costs)
+        if (item.partial && from == 0) {
+          const int at = position;
+          leave(a, item, -((at + span.tiles - 1) / chunk - static_cast<int>(blockIdx.x) + 1));
+        }
+        position = __builtin_amdgcn_readfirstlane(min(end, start + span.start + span.tiles + start_tiles(kKind)));
+        if (any) return true;
+        break;
+      }
+    }
+    return false;
+  }
+};
 
 // Rows are moved in 16-byte pieces, kPerRow of them to a row.
 template <int D, bool kE4M3>
@@ -222,15 +364,6 @@ __device__ __forceinline__ f32pair point_and_sum(float ref, float l) {
 }
 __device__ __forceinline__ float inverse(float l) { return l == 0.f ? 0.f : 1.f / l; }
 __device__ __forceinline__ float log_sum(float ref, float l) { return l == 0.f ? -INFINITY : ref * kLn2 + logf(l); }
-
-// This split's share of `tiles` key tiles.
-struct TileRange {
-  int begin, end;
-};
-__device__ __forceinline__ TileRange tile_range(const Item& item, int tiles) {
-  return TileRange{static_cast<int>(static_cast<int64_t>(tiles) * item.split / item.splits),
-                   static_cast<int>(static_cast<int64_t>(tiles) * (item.split + 1) / item.splits)};
-}
 
 }  // namespace
 }  // namespace cached

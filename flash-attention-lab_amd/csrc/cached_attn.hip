@@ -19,126 +19,126 @@ namespace fl {
 namespace cached {
 namespace {
 
-constexpr int kThreads = 256;
-
-// The partials of a row.
-struct Partials {
-  int splits;
-  int64_t first, step;  // rows of the workspace
-};
-__device__ __forceinline__ Partials partials_of(const CachedAttnArgs& a, const cache::Token& t, int head, int head_dim) {
-  const int2 info = a.sequence_splits[t.b];
-  const int hkv = head / a.group;
-  const int rows = t.count * a.group;
-  const int r = t.index * a.group + head - hkv * a.group;
-  const Kind kind = rows <= kNarrowRows ? kNarrow : kWide;
-  const int per_block = block_rows(kind, head_dim);
-  const int blocks = (rows + per_block - 1) / per_block;
-  const int block = r / per_block;
-  const int64_t slot = info.y + (static_cast<int64_t>(blocks - 1 - block) * a.c.heads_kv + hkv) * info.x;
-  return Partials{info.x, (kind == kWide ? a.wide_partials : 0) + slot * per_block + r - block * per_block, per_block};
-}
-
 // With M = max_s m_s, o = sum_s o_s 2^(m_s - M) / sum_s l_s 2^(m_s - M), the splits in a fixed order. Splits
-// in which a row sees no key (m = -inf) contribute nothing. kGroups groups of D / 4 lanes take every
-// kGroups-th split of a row and are added up in order through LDS: one for many rows of few splits, all of
-// a workgroup for few rows of many, where the time is that of one row's dependent loads.
-template <typename Tag, int D, int kGroups>
-__global__ void __launch_bounds__(kThreads) cached_merge_kernel(const CachedAttnArgs a) {
+// in which a row sees no key (m = -inf) contribute nothing. A workgroup takes 256 / (D / 4) rows of a
+// block, D / 4 lanes to a row; where a block has fewer rows than it has room for, several groups of lanes
+// share a row's splits and are added up in order through LDS. Bound by latency for few rows (list entry, then
+// partials), by reading the partials for many.
+constexpr int kMergeThreads = 256;
+template <int D>
+constexpr int kMergeRows = kMergeThreads / (D / 4);
+template <typename Tag, int D>
+__global__ void __launch_bounds__(kMergeThreads)
+    cached_merge_kernel(const CachedAttnArgs a, const MergeBlock* wide_blocks, int narrow_groups, int narrow_chunks) {
   using E = Elem<Tag>;
   constexpr int kLanes = D / 4;
-  constexpr int kRowThreads = kLanes * kGroups;
-  static_assert(kGroups == 1 || kRowThreads == kThreads, "a row's groups are a workgroup or one group");
-  const int64_t all = static_cast<int64_t>(a.c.tokens) * a.heads;
-  const int64_t at = (static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x) / kRowThreads;
-  const int64_t row = min(at, all - 1);
-  const int token = static_cast<int>(row / a.heads);
-  const int head = static_cast<int>(row - static_cast<int64_t>(token) * a.heads);
-  const cache::Token t = cache::find_token<kGroups == 1 ? kLanes : 64>(a.c, token);
-  if (at >= all || t.b < 0) return;
-  const Partials p = partials_of(a, t, head, D);
-  const int n = p.splits;
-  if (n <= 1) return;
+  constexpr int kGroups = kMergeRows<D>;
+  __shared__ f32x4 sums[kGroups][kLanes];
+  __shared__ float ls[kGroups];
+  const bool wide = static_cast<int>(blockIdx.x) >= narrow_groups;
+  const int id = wide ? blockIdx.x - narrow_groups : blockIdx.x;
+  const int chunks = wide ? block_rows(kWide, D) / kGroups : narrow_chunks;
+  const int at = id / chunks;
+  const int chunk = id - at * chunks;
+  const MergeBlock mb = (wide ? wide_blocks : a.merge_blocks)[at];
+  if (mb.splits == 0) return;
+  const int per_block = wide ? block_rows(kWide, D) : kNarrowRows;
+  const int rows = min(per_block, mb.count * a.group - mb.block * per_block);
+  const int first_row = chunk * kGroups;
+  if (first_row >= rows) return;
+  const int64_t base = wide ? a.wide_partials : 0;
+  const bool line = mb.splits < 0;
+  const int n = line ? -mb.splits : mb.splits;
+  auto slot_row = [&](int s) { return base + static_cast<int64_t>(line && s > 0 ? 2 * (at + s) : mb.slot + s) * per_block; };
   const int d = threadIdx.x % kLanes;
-  const int group = kGroups == 1 ? 0 : threadIdx.x / kLanes;
-  const f32pair* ml = a.partial_ml + p.first;
-  const f32x4* po = reinterpret_cast<const f32x4*>(a.partial_o + p.first * D) + d;
+  const int group = threadIdx.x / kLanes;
+  // Groups to a row (a power of two), where all of the chunk's rows fit.
+  int share = 1;
+  while (!wide && 2 * share * min(rows - first_row, kGroups) <= kGroups) share *= 2;
+  const int part = group & (share - 1);
+  const int r = first_row + group / share;
+  const bool in = r < rows;
+  auto row_of = [&](int s) { return slot_row(s) + (in ? r : 0); };
   float m = -INFINITY;
-  if constexpr (kGroups == 1) {
-    for (int s = 0; s < n; ++s) m = fmaxf(m, ml[s * p.step].x);
-  } else {
-    for (int s = threadIdx.x & 63; s < n; s += 64) m = fmaxf(m, ml[s * p.step].x);
-#pragma unroll
-    for (int k = 32; k >= 1; k /= 2) m = fmaxf(m, __shfl_xor(m, k));
-  }
   float l = 0.f;
   f32x4 o = {};
+  // The first two partials of a lane are on their way before any maximum is known.
+  const int s0 = part, s1 = part + share;
+  const bool has0 = s0 < n, has1 = s1 < n;
+  const f32x4 o0 = has0 ? reinterpret_cast<const f32x4*>(a.partial_o + row_of(s0) * D)[d] : f32x4{};
+  const f32x4 o1 = has1 ? reinterpret_cast<const f32x4*>(a.partial_o + row_of(s1) * D)[d] : f32x4{};
 #pragma unroll 4
-  for (int s = group; s < n; s += kGroups) {
-    const f32pair x = ml[s * p.step];
-    const float f = x.x == -INFINITY ? 0.f : exp2_fast(x.x - m);
-    l += x.y * f;
-    o += po[s * p.step * kLanes] * f;
-  }
-  if constexpr (kGroups > 1) {
-    __shared__ f32x4 sums[kGroups][kLanes];
-    __shared__ float ls[kGroups];
+  for (int s = 0; s < n; ++s) m = fmaxf(m, a.partial_ml[row_of(s)].x);
+  auto add = [&](int s, const f32x4& x) {
+    const f32pair p = a.partial_ml[row_of(s)];
+    const float f = p.x == -INFINITY ? 0.f : exp2_fast(p.x - m);
+    l += p.y * f;
+    o += x * f;
+  };
+  if (has0) add(s0, o0);
+  if (has1) add(s1, o1);
+#pragma unroll 4
+  for (int s = s1 + share; s < n; s += share) add(s, reinterpret_cast<const f32x4*>(a.partial_o + row_of(s) * D)[d]);
+  if (share > 1) {
     sums[group][d] = o;
     if (d == 0) ls[group] = l;
     __syncthreads();
-    if (group != 0) return;
-#pragma unroll
-    for (int k = 1; k < kGroups; ++k) {
-      o += sums[k][d];
-      l += ls[k];
+    if (part != 0) return;
+    for (int k = 1; k < share; ++k) {
+      o += sums[group + k][d];
+      l += ls[group + k];
     }
   }
+  if (!in) return;
   const float inv = inverse(l);
-  const int64_t base = a.c.cu_seqlens ? token * a.o_ss : t.b * a.o_bs + t.index * a.o_ss;
-  *reinterpret_cast<u32x2*>(a.o + base + head * a.o_hs + 4 * d) =
+  const int place = mb.block * per_block + r;
+  const int token = token_of_row(a, place);
+  const int head = mb.hkv * a.group + place - token * a.group;
+  const int64_t o_row = a.c.cu_seqlens ? (mb.start + token) * a.o_ss : mb.b * a.o_bs + token * a.o_ss;
+  *reinterpret_cast<u32x2*>(a.o + o_row + head * a.o_hs + 4 * d) =
       u32x2{E::pack2(o[0] * inv, o[1] * inv), E::pack2(o[2] * inv, o[3] * inv)};
-  if (d == 0) a.lse[row] = log_sum(m, l);
+  if (d == 0) a.lse[(static_cast<int64_t>(mb.start) + token) * a.heads + head] = log_sum(m, l);
 }
 
 template <typename Tag, int D>
 hipError_t launch_merge(const CachedAttnArgs& args, const CachedPlan& plan, hipStream_t stream) {
-  const int64_t rows = static_cast<int64_t>(args.c.tokens) * args.heads;
-  if (plan.many_splits) {
-    hipLaunchKernelGGL((cached_merge_kernel<Tag, D, kThreads / (D / 4)>), dim3(static_cast<uint32_t>(rows)),
-                       dim3(kThreads), 0, stream, args);
-  } else {
-    const int64_t lanes = rows * (D / 4);
-    hipLaunchKernelGGL((cached_merge_kernel<Tag, D, 1>), dim3(static_cast<uint32_t>((lanes + kThreads - 1) / kThreads)),
-                       dim3(kThreads), 0, stream, args);
-  }
+  const int most = plan.most_rows < kNarrowRows ? plan.most_rows : kNarrowRows;
+  const int narrow_chunks = (most + kMergeRows<D> - 1) / kMergeRows<D>;
+  const int narrow_groups = plan.narrow.merges * narrow_chunks;
+  const int wide_groups = plan.wide.merges * (block_rows(kWide, D) / kMergeRows<D>);
+  hipLaunchKernelGGL((cached_merge_kernel<Tag, D>), dim3(narrow_groups + wide_groups), dim3(kMergeThreads), 0, stream,
+                     args, args.merge_blocks + plan.narrow.merges, narrow_groups, narrow_chunks);
   return hipGetLastError();
 }
 
-// Grid, slots and rounds of one kind's kernel, whose sequences have `least` to `most` blocks in all and run
-// on `slots` workgroups at once.
-CachedPlan::Part plan_part(const CachedAttnArgs& args, int64_t least, int64_t most, int64_t resident, int min_tiles) {
+// Grid and slots of one kind's kernel, whose sequences have `least` to `most` blocks in all and which runs
+// `resident` workgroups at once (Segments, cached.hpp).
+CachedPlan::Part plan_part(const CachedAttnArgs& args, Kind kind, int64_t least, int64_t most, int64_t resident,
+                           int min_tiles, bool whole) {
   CachedPlan::Part part{};
   part.workgroups = most;
   part.min_tiles = min_tiles;
-  part.max_rounds = 1;
   const int64_t tiles = (args.c.capacity + kKeys - 1) / kKeys;
   if (args.num_splits > 1) {
-    part.workgroups = part.partials = most * args.num_splits;
-  } else if (args.num_splits == 0 && tiles > min_tiles && least < kMaxRounds * resident) {
+    part.workgroups = part.partials = part.merges = most * args.num_splits;
+  } else if (args.num_splits == 0 && tiles > min_tiles && least <= kWholeRounds * resident && !whole) {
     part.slots = static_cast<int>(resident);
-    // (With few blocks one round of splits is even enough.)
-    part.max_rounds = 4 * most <= resident ? 1 : kMaxRounds;
-    const int64_t splits = (tiles + min_tiles - 1) / min_tiles;
-    const int64_t items = part.max_rounds * resident;
-    part.partials = most * splits < items ? most * splits : items;
-    part.workgroups = part.partials > most ? part.partials : most;
+    // The line needs blocks enough, and positions that fit 32 bits.
+    part.line = kind == kWide && 4 * most > resident && most * (tiles + start_tiles(kind) + 1) < (int64_t{1} << 30);
+    const int64_t shares = most * ((tiles + min_tiles - 1) / min_tiles);
+    part.partials = part.line ? 2 * resident : shares < resident ? shares : resident;
+    part.workgroups = part.line || part.partials == resident ? resident : part.partials;
+    if (most > part.workgroups) part.workgroups = most;
+    part.merges = static_cast<int>(part.line ? resident : part.partials);
   }
   return part;
 }
 
-CachedAttnArgs with_part(CachedAttnArgs args, const CachedPlan::Part& part) {
+CachedAttnArgs with_part(CachedAttnArgs args, const CachedPlan::Part& part, int64_t blocks_before) {
+  args.merge_blocks += blocks_before;
+  args.merges = part.merges;
   args.slots = part.slots;
-  args.max_rounds = part.max_rounds;
+  args.line = part.line;
   args.min_tiles = part.min_tiles;
   return args;
 }
@@ -156,10 +156,15 @@ CachedPlan plan_cached_attn(const CachedAttnArgs& args, int head_dim, bool e4m3,
   CachedPlan plan{};
   // Rows of the largest sequence there can be, which kinds there can be, and their blocks.
   plan.most_rows = static_cast<int>(ragged ? rows : per_seq);
+  // Short caches of one kind keep their blocks whole: a workgroup takes about 7.2 us for 1,000 keys, the merge and
+  // its launch 6.4 us and more with what else is read (one split / several, e4m3: B = 1, 32/8 heads, 640 keys 10.4
+  // us / 6.9 + 4.7, 1,024 13.6 / 7.0 + 4.6; B = 16, 1,024 keys 17.5 / 13.3 + 4.2, 1,536 22.5 / 15.3 + 4.1).
+  const double megabytes = 2e-6 * c.batch * c.heads_kv * c.capacity * head_dim * (e4m3 ? 1 : 2);
+  const bool whole = plan.most_rows <= kNarrowRows && 7.2e-3 * c.capacity < 6.4 + 0.08 * megabytes;
   if (ragged || per_seq <= kNarrowRows) {
     const int64_t least = ragged ? 0 : c.batch * int64_t{c.heads_kv};
-    plan.narrow = plan_part(args, least, c.batch * int64_t{c.heads_kv},
-                            cus * cached_narrow_resident(head_dim, e4m3, plan.most_rows), 2);
+    plan.narrow = plan_part(args, kNarrow, least, c.batch * int64_t{c.heads_kv},
+                            cus * cached_narrow_resident(head_dim, e4m3, plan.most_rows), 2, whole);
   }
   if (plan.most_rows > kNarrowRows) {
     const int64_t wide_rows = block_rows(kWide, head_dim);
@@ -167,13 +172,12 @@ CachedPlan plan_cached_attn(const CachedAttnArgs& args, int head_dim, bool e4m3,
     const int64_t least = ragged ? 0 : blocks * c.heads_kv;
     const int64_t most = (ragged ? rows / wide_rows + (c.batch < rows / kNarrowRows + 1 ? c.batch : rows / kNarrowRows + 1)
                                  : blocks) * c.heads_kv;
-    plan.wide = plan_part(args, least, most, wide_resident(head_dim) * cus, 4);
+    plan.wide = plan_part(args, kWide, least, most, wide_resident(head_dim) * cus, 4, false);
   }
   plan.wide_partials = plan.narrow.partials * kNarrowRows;
   plan.partial_rows = plan.wide_partials + plan.wide.partials * block_rows(kWide, head_dim);
-  if (plan.partial_rows > 0) plan.floats = plan.partial_rows * (head_dim + 2) + 2 * static_cast<int64_t>(c.batch);
-  // One workgroup per row pays while the rows are about as few as the CUs and their splits many.
-  plan.many_splits = static_cast<int64_t>(c.tokens) * args.heads <= 8 * cus;
+  plan.floats = plan.partial_rows * (head_dim + 2) +
+                (plan.narrow.merges + static_cast<int64_t>(plan.wide.merges)) * (sizeof(MergeBlock) / sizeof(float));
   return plan;
 }
 
@@ -182,9 +186,9 @@ hipError_t launch_cached_attn(const CachedAttnArgs& args, const CachedPlan& plan
   using namespace cached;
   hipError_t err = hipSuccess;
   if (plan.wide.workgroups > 0)
-    err = launch_cached_wide(with_part(args, plan.wide), plan.wide.workgroups, dtype, e4m3, head_dim, stream);
+    err = launch_cached_wide(with_part(args, plan.wide, plan.narrow.merges), plan.wide.workgroups, dtype, e4m3, head_dim, stream);
   if (err == hipSuccess && plan.narrow.workgroups > 0)
-    err = launch_cached_narrow(with_part(args, plan.narrow), plan, dtype, e4m3, head_dim, stream);
+    err = launch_cached_narrow(with_part(args, plan.narrow, 0), plan, dtype, e4m3, head_dim, stream);
   if (err != hipSuccess || plan.partial_rows == 0) return err;
   if (head_dim == 64) {
     return dtype == DType::bf16 ? launch_merge<bf16_tag, 64>(args, plan, stream)

@@ -88,10 +88,9 @@ __device__ __forceinline__ void narrow_item(const CachedAttnArgs& a, const Item&
   const int rows = seq.count * a.group;  // <= 16 kCols
   const int offset = seq.len - seq.count;
   const int last = seq.len - 1;
-  const TileRange range = tile_range(item, (seq.len + kKeys - 1) / kKeys);
   // In tiles of 32 keys.
-  const int begin = 2 * range.begin + wave;
-  const int end = min(2 * range.end, (seq.len + kTileKeys - 1) / kTileKeys);
+  const int begin = 2 * item.begin + wave;
+  const int end = min(2 * item.end, (seq.len + kTileKeys - 1) / kTileKeys);
   const int tiles = end > begin ? (end - begin + kWaves - 1) / kWaves : 0;
 
   char* work = smem + kQBytes<D, kCols>;
@@ -304,7 +303,7 @@ __device__ __forceinline__ void narrow_item(const CachedAttnArgs& a, const Item&
         den += x.y * f;
       }
       const int row = 16 * c + r;
-      if (item.splits > 1) {
+      if (item.partial) {
         const int64_t slot_row = static_cast<int64_t>(item.slot) * kNarrowRows + row;
         *reinterpret_cast<f32x4*>(a.partial_o + slot_row * D + d) = num;
         if (d == 0) a.partial_ml[slot_row] = f32pair{m, den};
@@ -352,10 +351,10 @@ __global__ void __launch_bounds__(kThreads)
     cached_narrow_kernel(const CachedAttnArgs a) {
   __shared__ __attribute__((aligned(16))) char smem[kQBytes<D, kCols> + kWorkBytes<D>];
   clear_unowned<D>(a);
+  Segments<kNarrow, D> segments(a);
   Item item;
-  if (!find_item<kNarrow, D>(a, blockIdx.x, item)) return;
-  if (item.first && threadIdx.x == 0 && a.sequence_splits != nullptr)
-    a.sequence_splits[item.b] = int2{item.splits, item.first_slot};
+  if (!segments.next(a, item)) return;
+  item = uniform(item);
   if (kMixed && item.seq.count * a.group <= 16) {
     narrow_item<Tag, D, kE4M3, 1>(a, item, smem);
   } else {

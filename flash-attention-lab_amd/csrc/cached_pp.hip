@@ -47,30 +47,31 @@ constexpr int kAhead = 2;   // fragments read ahead of their MFMAs
 // What V's rows behind a sequence's last one are read as.
 __device__ const u32x4 zero_row[D * 2 / 16] = {};
 
+template <bool kE4M3>
+constexpr int kSmemBytes = 4 * kStagesOf<kE4M3> * kTileElems<D> + (kE4M3 ? 2 * kWaves * 16 * D : 0);
+
 template <typename Tag, bool kE4M3>
-__global__ void __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2, 2)))
-    cached_pp_kernel(const CachedAttnArgs a) {
+__device__ __forceinline__ void pp_item(const CachedAttnArgs& a, const Item& item, uint16_t* smem) {
   using E = Elem<Tag>;
   using P = Piece<D, kE4M3>;
   constexpr int kStages = kStagesOf<kE4M3>;
-  constexpr int kTile = kTileElems<D>;
-  constexpr int kSlotBytes = 2 * kTile;
+  constexpr int kSlotBytes = 2 * kTileElems<D>;
   constexpr int kVRingBytes = kStages * kSlotBytes;
   constexpr int kCodeBytes = kE4M3 ? 16 * D : 0;  // a wave's rows of a tile, as codes
   constexpr int kCodesAt = 2 * kVRingBytes;
-  __shared__ __attribute__((aligned(16))) uint16_t smem[(kCodesAt + 2 * kWaves * kCodeBytes) / 2];
+  constexpr int kSmem = kSmemBytes<kE4M3>;
+  static_assert(kSmem == kCodesAt + 2 * kWaves * kCodeBytes, "two tiles' codes");
   const char* lds_bytes = reinterpret_cast<const char*>(smem);
 
-  const int tid = threadIdx.x;
+  // (Opaque: what follows from it is worked out again for every item instead of being kept, which took 127 more
+  // registers than there are.)
+  int tid = threadIdx.x;
+  asm volatile("" : "+v"(tid));
   const int lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int group = wave >> 2;
   const int half = lane >> 5;
 
-  Item item;
-  if (!find_item<kWide, D>(a, blockIdx.x, item)) return;
-  if (item.first && tid == 0 && a.sequence_splits != nullptr)
-    a.sequence_splits[item.b] = int2{item.splits, item.first_slot};
   const Sequence& seq = item.seq;
   const int rows = seq.count * a.group;
   const int q0 = item.block * kRows;
@@ -78,12 +79,9 @@ __global__ void __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2
   const int my_row = row0 + (lane & 31);
   const int last = seq.len - 1;
 
-  // Keys of the block, and this split's tiles. Keys and positions count from its first tile.
-  int kv_end = seq.len;
-  if (a.causal) kv_end = min(kv_end, token_of_row(a, min(q0 + kRows, rows) - 1) + 1 + seq.len - seq.count);
-  const TileRange range = tile_range(item, kv_end > 0 ? (kv_end + kKeys - 1) / kKeys : 0);
-  const int num_tiles = range.end - range.begin;
-  const int key0 = range.begin * kKeys;
+  // Keys and positions count from the item's first tile.
+  const int num_tiles = item.end - item.begin;
+  const int key0 = item.begin * kKeys;
   const int offset = seq.len - seq.count - key0;
   const int seqlen_k = seq.len - key0;
   // Tiles this wave sees any key of, and the first whose scores need masking.
@@ -423,12 +421,11 @@ __global__ void __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2
   phase_barrier();
   // Rows leave whole: each wave stages its 32 in its own part of the (free) rings, padded by 16 bytes.
   const float lt = sum_halves(l);
-  const bool partial = item.splits > 1;
-  constexpr int kStageRow = 4 * D + 16;
-  static_assert(kWaves * 16 * kStageRow <= static_cast<int>(sizeof(smem)), "16 rows of each wave fit");
+    constexpr int kStageRow = 4 * D + 16;
+  static_assert(kWaves * 16 * kStageRow <= kSmem, "16 rows of each wave fit");
   char* stage = reinterpret_cast<char*>(smem) + wave * 16 * kStageRow;
   const float inv = inverse(lt);
-  if (partial) {
+  if (item.partial) {
     // (In two halves of 16 rows.)
     float* po = a.partial_o + (a.wide_partials + static_cast<int64_t>(item.slot) * kRows + wave * kWaveRows) * D;
 #pragma unroll
@@ -482,6 +479,18 @@ __global__ void __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2
     const int token = token_of_row(a, my_row);
     a.lse[(static_cast<int64_t>(seq.start) + token) * a.heads + item.hkv * a.group + my_row - token * a.group] =
         log_sum(ref, lt);
+  }
+}
+
+template <typename Tag, bool kE4M3>
+__global__ void __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2, 2)))
+    cached_pp_kernel(const CachedAttnArgs a) {
+  __shared__ __attribute__((aligned(16))) uint16_t smem[kSmemBytes<kE4M3> / 2];
+  Segments<kWide, D> segments(a);
+  Item item;
+  while (segments.next(a, item)) {
+    pp_item<Tag, kE4M3>(a, uniform(item), smem);
+    phase_barrier();  // (the next item uses the LDS again)
   }
 }
 

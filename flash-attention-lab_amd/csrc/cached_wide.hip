@@ -9,6 +9,7 @@
 //    conversion instruction with the scale in it (exact in bf16). So the matrix cores see the tokens' type
 //    whatever the cache holds, and a row's codes are converted once per workgroup.
 #include "cached.hpp"
+#include "prefill_pp.hpp"
 
 namespace fl {
 namespace cached {
@@ -25,6 +26,7 @@ using prefill::p_frag;
 using prefill::tile_offset;
 using prefill::v_frag_at;
 using prefill::v_lane_offset;
+using prefill::pp::phase_barrier;
 
 constexpr int kWaves = 4;
 constexpr int kThreads = 64 * kWaves;
@@ -57,7 +59,10 @@ __device__ __forceinline__ void wide_item(const CachedAttnArgs& a, const Item& i
   auto k_lds = [&](int slot) { return smem + slot * kTile; };
   auto v_lds = [&](int slot) { return smem + (2 + slot) * kTile; };
 
-  const int tid = threadIdx.x;
+  // (Opaque: what follows from it is worked out again for every item instead of being kept, which took 127 more
+  // registers than there are.)
+  int tid = threadIdx.x;
+  asm volatile("" : "+v"(tid));
   const int lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int half = lane >> 5;
@@ -71,13 +76,8 @@ __device__ __forceinline__ void wide_item(const CachedAttnArgs& a, const Item& i
   const int my_head = item.hkv * a.group + my_row - my_token * a.group;
   const bool mine = my_row < rows;
 
-  // Keys of the block, and this split's tiles of them.
-  int kv_end = seq.len;
-  if (a.causal)
-    kv_end = min(kv_end, token_of_row(a, min(item.block * kRows + kRows, rows) - 1) + 1 + offset);
-  const int all_tiles = kv_end > 0 ? (kv_end + kKeys - 1) / kKeys : 0;
-  const auto [t_begin, t_end] = tile_range(item, all_tiles);
-
+  const int t_begin = item.begin;
+  const int t_end = item.end;
   const int64_t q_base = a.c.cu_seqlens ? seq.start * a.q_ss : item.b * a.q_bs;
   u32x4 qf[D / 16];
   {
@@ -175,6 +175,14 @@ __device__ __forceinline__ void wide_item(const CachedAttnArgs& a, const Item& i
       s0 = E::mfma32(prefill::lds_load16(kt, k_off[ks]), qf[ks], s0);
       s1 = E::mfma32(prefill::lds_load16(kt + kKeyBlockBytes<D>, k_off[ks]), qf[ks], s1);
     }
+    // (K fragments two steps ahead of their MFMAs: prefill_fwd.hip)
+    __builtin_amdgcn_sched_group_barrier(0x100, 4, 1);
+#pragma unroll
+    for (int ks = 0; ks < D / 16 - 2; ++ks) {
+      __builtin_amdgcn_sched_group_barrier(0x008, 2, 1);
+      __builtin_amdgcn_sched_group_barrier(0x100, 2, 1);
+    }
+    __builtin_amdgcn_sched_group_barrier(0x008, 4, 1);
     if (k0 + kKeys - 1 > first_limit) {
       const int lim = last_key - k0 - 4 * half;
 #pragma unroll
@@ -243,12 +251,12 @@ __device__ __forceinline__ void wide_item(const CachedAttnArgs& a, const Item& i
       locate(t + 3, at, byte);
       at = find(t + 4);
       tile_step(t, t & 1);
-      __syncthreads();
+      phase_barrier();  // (the loads in flight need not have come back)
     }
   }
 
   const float lt = sum_halves(l);
-  if (item.splits > 1) {
+  if (item.partial) {
     if (mine) {
       const int64_t slot_row = a.wide_partials + static_cast<int64_t>(item.slot) * kRows + wave * kWaveRows + (lane & 31);
       float* po = a.partial_o + slot_row * D + 4 * half;
@@ -284,11 +292,12 @@ template <typename Tag, int D, bool kE4M3>
 __global__ void __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2, 2)))
     cached_wide_kernel(const CachedAttnArgs a) {
   __shared__ __attribute__((aligned(16))) uint16_t smem[4 * kTileElems<D> + 4 * kKeys * (8 + 4) / 2];
+  Segments<kWide, D> segments(a);
   Item item;
-  if (!find_item<kWide, D>(a, blockIdx.x, item)) return;
-  if (item.first && threadIdx.x == 0 && a.sequence_splits != nullptr)
-    a.sequence_splits[item.b] = int2{item.splits, item.first_slot};
-  wide_item<Tag, D, kE4M3>(a, item, smem);
+  while (segments.next(a, item)) {
+    wide_item<Tag, D, kE4M3>(a, uniform(item), smem);
+    __syncthreads();  // (the next item uses the LDS again)
+  }
 }
 
 template <typename Tag, int D>

@@ -123,6 +123,12 @@ struct TokenRows {
   int64_t v_bs, v_ss, v_hs;
 };
 
+// A block of rows whose partials are merged: `splits` of them in consecutive slots from `slot` on, or, negative,
+// the first in `slot` and partial s in slot 2 (w + s), w being the entry's place in the list. 0: none.
+struct MergeBlock {
+  int splits, slot, b, hkv, block, start, count, unused;
+};
+
 struct CachedAttnArgs {
   CacheArgs c;
   const uint16_t* q;
@@ -138,14 +144,15 @@ struct CachedAttnArgs {
   int num_splits;  // forced, or 0
   // Of the kind of sequences that a kernel runs (cached.hpp):
   int slots;       // workgroups that run at once, where keys may be split; 0: no splits
-  int max_rounds;  // of slots workgroups each
+  int line;        // whether they may share a line (cached.hpp)
   int min_tiles;   // fewest key tiles of a split
   // Partials: [slot][row of the block], the narrow sequences' slots first, the wide ones' from row
   // wide_partials on.
   int64_t wide_partials;
   float* partial_o;       // [D] unnormalized
   f32pair* partial_ml;    // (reference point in log2 units or -inf, sum)
-  int2* sequence_splits;  // [B] (splits, first slot) of the sequences with tokens
+  MergeBlock* merge_blocks;  // of this kind
+  int merges;
 };
 
 // How the decode kernels find cache rows: contiguous cache, paged cache with the split's block
@@ -221,15 +228,14 @@ hipError_t launch_cache_read(const CacheArgs& args, const TokenRows& rows, DType
                              int head_dim, hipStream_t stream);
 
 // Attention over a cache (cached_attn.hip): how a call is launched, and the floats of its workspace
-// (partial_o, then partial_ml, then sequence_splits).
+// (partial_o, then partial_ml, then the narrow and the wide merge_blocks).
 struct CachedPlan {
   struct Part {
     int64_t workgroups, partials;  // of the grid, slots of partials
-    int slots, max_rounds, min_tiles;
+    int slots, line, min_tiles, merges;
   };
   Part narrow, wide;  // workgroups 0: there are none of the kind
   int most_rows;      // of a sequence
-  bool many_splits;   // few rows
   int64_t wide_partials, partial_rows, floats;
 };
 CachedPlan plan_cached_attn(const CachedAttnArgs& args, int head_dim, bool e4m3, int cu_count);
