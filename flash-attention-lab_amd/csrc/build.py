@@ -31,7 +31,7 @@ OUTPUT = PKG_ROOT / "flash_lab" / "libflash_lab_hip.so"
 
 SOURCES = ("abi.hip", "prefill_fwd.hip", "prefill_pp.hip", "prefill_causal.hip", "decode.hip",
            "decode_mfma.hip", "cache.hip", "cached_attn.hip", "cached_narrow.hip",
-           "cached_pp.hip", "cached_wide.hip", "smoke.hip")
+           "cached_wide.hip", "smoke.hip")
 TORCH_SOURCE = "torch_ops.cpp"
 TORCH_OUTPUT = PKG_ROOT / "flash_lab" / "libflash_lab_torch.so"
 ARCH = "gfx950"

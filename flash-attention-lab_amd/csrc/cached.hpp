@@ -1,6 +1,6 @@
 // Pieces shared by the kernels of attention over a cache (cached_attn.hip: plan and merge; cached_narrow.hip:
-// sequences with few rows; cached_pp.hip and cached_wide.hip: the
-// others, at head_dim 128 and 64): the rows of a sequence, the items that the
+// sequences with few rows; cached_wide.hip: the
+// others): the rows of a sequence, the items that the
 // workgroups of a kernel share out, and the offsets of cache rows.
 #pragma once
 
@@ -22,11 +22,7 @@ __host__ __device__ __forceinline__ constexpr int start_tiles(Kind kind) { retur
 // From so many rounds of blocks on they run whole, as they come, the longest first.
 constexpr int kWholeRounds = 6;
 // Rows of a block.
-__host__ __device__ __forceinline__ constexpr int block_rows(Kind kind, int head_dim) {
-  return kind == kNarrow ? kNarrowRows : head_dim == 128 ? 256 : 128;
-}
-// Workgroups of the wide kernel per CU.
-constexpr int wide_resident(int head_dim) { return head_dim == 128 ? 1 : 2; }
+__host__ __device__ __forceinline__ constexpr int block_rows(Kind kind) { return kind == kNarrow ? kNarrowRows : 256; }
 
 namespace {
 
@@ -79,7 +75,7 @@ template <Kind kKind, int D>
 __device__ __forceinline__ int blocks_of(const CachedAttnArgs& a, const Sequence& s) {
   const int rows = s.count * a.group;
   const bool mine = (rows <= kNarrowRows) == (kKind == kNarrow);
-  return mine ? (rows + block_rows(kKind, D) - 1) / block_rows(kKind, D) : 0;
+  return mine ? (rows + block_rows(kKind) - 1) / block_rows(kKind) : 0;
 }
 __device__ __forceinline__ int tiles_of(const Sequence& s) { return (s.len + kKeys - 1) / kKeys; }
 // Key tiles that block i of a sequence sees any key of.
@@ -87,7 +83,7 @@ template <Kind kKind, int D>
 __device__ __forceinline__ int block_tiles(const CachedAttnArgs& a, const Sequence& s, int i) {
   int end = s.len;
   if (a.causal) {
-    const int rows = min((i + 1) * block_rows(kKind, D), s.count * a.group);
+    const int rows = min((i + 1) * block_rows(kKind), s.count * a.group);
     end = max(min(end, token_of_row(a, max(rows - 1, 0)) + 1 + s.len - s.count), 0);
   }
   return (end + kKeys - 1) / kKeys;

@@ -9,7 +9,7 @@
 //
 // Lengths are known on the device only. Sequences with few rows (tokens x heads of a group) are bound by
 // reading the cache and run on cached_narrow.hip, those with many by the matrix cores and run on
-// cached_pp.hip (head_dim 128) or cached_wide.hip (64); without cu_seqlens the host knows which it is, and only that kernel is launched.
+// cached_wide.hip; without cu_seqlens the host knows which it is, and only that kernel is launched.
 // Every workgroup of either derives the same list of items from the lengths (find_item, cached.hpp) and
 // takes the one of its own number; the grid is an upper bound from the sizes. Where the items are few, keys
 // are split over several workgroups, and a last kernel, here, merges the partials in order.
@@ -37,12 +37,12 @@ __global__ void __launch_bounds__(kMergeThreads)
   __shared__ float ls[kGroups];
   const bool wide = static_cast<int>(blockIdx.x) >= narrow_groups;
   const int id = wide ? blockIdx.x - narrow_groups : blockIdx.x;
-  const int chunks = wide ? block_rows(kWide, D) / kGroups : narrow_chunks;
+  const int chunks = wide ? block_rows(kWide) / kGroups : narrow_chunks;
   const int at = id / chunks;
   const int chunk = id - at * chunks;
   const MergeBlock mb = (wide ? wide_blocks : a.merge_blocks)[at];
   if (mb.splits == 0) return;
-  const int per_block = wide ? block_rows(kWide, D) : kNarrowRows;
+  const int per_block = wide ? block_rows(kWide) : kNarrowRows;
   const int rows = min(per_block, mb.count * a.group - mb.block * per_block);
   const int first_row = chunk * kGroups;
   if (first_row >= rows) return;
@@ -105,7 +105,7 @@ hipError_t launch_merge(const CachedAttnArgs& args, const CachedPlan& plan, hipS
   const int most = plan.most_rows < kNarrowRows ? plan.most_rows : kNarrowRows;
   const int narrow_chunks = (most + kMergeRows<D> - 1) / kMergeRows<D>;
   const int narrow_groups = plan.narrow.merges * narrow_chunks;
-  const int wide_groups = plan.wide.merges * (block_rows(kWide, D) / kMergeRows<D>);
+  const int wide_groups = plan.wide.merges * (block_rows(kWide) / kMergeRows<D>);
   hipLaunchKernelGGL((cached_merge_kernel<Tag, D>), dim3(narrow_groups + wide_groups), dim3(kMergeThreads), 0, stream,
                      args, args.merge_blocks + plan.narrow.merges, narrow_groups, narrow_chunks);
   return hipGetLastError();
@@ -167,15 +167,15 @@ CachedPlan plan_cached_attn(const CachedAttnArgs& args, int head_dim, bool e4m3,
                             cus * cached_narrow_resident(head_dim, e4m3, plan.most_rows), 2, whole);
   }
   if (plan.most_rows > kNarrowRows) {
-    const int64_t wide_rows = block_rows(kWide, head_dim);
+    const int64_t wide_rows = block_rows(kWide);
     const int64_t blocks = (per_seq + wide_rows - 1) / wide_rows * c.batch;
     const int64_t least = ragged ? 0 : blocks * c.heads_kv;
     const int64_t most = (ragged ? rows / wide_rows + (c.batch < rows / kNarrowRows + 1 ? c.batch : rows / kNarrowRows + 1)
                                  : blocks) * c.heads_kv;
-    plan.wide = plan_part(args, kWide, least, most, wide_resident(head_dim) * cus, 4, false);
+    plan.wide = plan_part(args, kWide, least, most, cus, 4, false);
   }
   plan.wide_partials = plan.narrow.partials * kNarrowRows;
-  plan.partial_rows = plan.wide_partials + plan.wide.partials * block_rows(kWide, head_dim);
+  plan.partial_rows = plan.wide_partials + plan.wide.partials * block_rows(kWide);
   plan.floats = plan.partial_rows * (head_dim + 2) +
                 (plan.narrow.merges + static_cast<int64_t>(plan.wide.merges)) * (sizeof(MergeBlock) / sizeof(float));
   return plan;

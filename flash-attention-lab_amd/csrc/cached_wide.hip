@@ -1,13 +1,17 @@
-// Attention over a cache for sequences with many rows (fl_cached_attention, cached.hpp): chunks of prompts.
-// One pass over the keys with a running reference point and sum per row, on the lane layouts of
-// prefill_tile.hpp (scores and outputs transposed, a lane per query row).
+// Attention over a cache for sequences with many rows (fl_cached_attention, cached.hpp): chunks
+// of prompts, bound by the matrix cores. The arithmetic, lane layouts and phases are those of the prefill
+// kernel (prefill_pp.hip): 8 waves of 32 rows, two to a SIMD in two groups that take turns, one group's
+// MFMAs running beside the other's softmax, one barrier per tile of 64 keys. What differs is where keys
+// come from and how the work is found:
 //
-//  * The query heads of a KV head are packed: row r of a sequence is token r / group, head r % group. A
-//    workgroup has 4 waves of 32 rows and streams key tiles of 64 through LDS, two slots each for K and V.
-//  * Tiles go through registers: a thread loads 16-byte pieces of the tile after the next one and, an
-//    iteration later, puts them into the other slot; codes become bf16 or fp16 on the way, pairs per
-//    conversion instruction with the scale in it (exact in bf16). So the matrix cores see the tokens' type
-//    whatever the cache holds, and a row's codes are converted once per workgroup.
+//  * Rows may lie anywhere (a pool's blocks of any size). Group 0 moves K, group 1 V, 16 rows a wave, in its
+//    MFMA phase, between the MFMAs: one lane works out a row's address, the lanes that move its 16-byte
+//    pieces get it by a lane permute. In period m they ask for tile m + 2, so a load has a whole period (about
+//    2,000 cycles) to come back. Rows in the tokens' type go straight into LDS; codes go through registers,
+//    and a period later become the tokens' type (a pair per instruction, scale included) and go into LDS, once
+//    per workgroup.
+//  * A workgroup has one item, a share of a block's tiles (cached.hpp), and the rows of all query heads of
+//    a KV head.
 #include "cached.hpp"
 #include "prefill_pp.hpp"
 
@@ -28,36 +32,45 @@ using prefill::v_frag_at;
 using prefill::v_lane_offset;
 using prefill::pp::phase_barrier;
 
-constexpr int kWaves = 4;
+constexpr int kWaves = 8;
 constexpr int kThreads = 64 * kWaves;
 constexpr int kWaveRows = 32;
-constexpr int kRows = block_rows(kWide, 64);
-static_assert(kRows == kWaves * kWaveRows, "a wave per 32 rows");
+constexpr int kRows = kWaves * kWaveRows;
+static_assert(kRows == block_rows(kWide), "a wave per 32 rows");
+// LDS slots for K and for V: in period m the tiles m - 1 (V), m and m + 1, and in the tokens' type one more that
+// loads bring in (codes arrive in a place of their own, where they are three tiles).
+template <bool kE4M3>
+constexpr int kStagesOf = kE4M3 ? 3 : 4;
+constexpr int kAhead = 2;        // fragments read ahead of their MFMAs
+constexpr int kTableEntries = 2048;  // of the block table that an item keeps in LDS
 
-// A piece into a tile in LDS, as Tag's elements.
-template <typename Tag, int D, bool kE4M3>
-__device__ __forceinline__ void put_piece(uint16_t* tile, int row, int col, const u32x4& piece, float scale) {
-  if constexpr (kE4M3) {
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const u32x2 lo = cache::values4<Tag>(piece[2 * h], scale);
-      const u32x2 hi = cache::values4<Tag>(piece[2 * h + 1], scale);
-      *reinterpret_cast<u32x4*>(tile + tile_offset<D>(row, col + 8 * h)) = u32x4{lo[0], lo[1], hi[0], hi[1]};
-    }
-  } else {
-    *reinterpret_cast<u32x4*>(tile + tile_offset<D>(row, col)) = piece;
-  }
-}
+// LDS: the K ring, the V ring, each wave's codes of three tiles and their scales, and the item's part of the
+// block table.
+template <int D, bool kE4M3>
+struct Lds {
+  static constexpr int kSlotBytes = 2 * kTileElems<D>;
+  static constexpr int kRingBytes = kStagesOf<kE4M3> * kSlotBytes;
+  static constexpr int kCodeBytes = 16 * D;    // a wave's rows of a tile, as codes
+  static constexpr int kScaleBytes = 64 * 4;
+  static constexpr int kCodes = 2 * kRingBytes;
+  static constexpr int kScales = kCodes + (kE4M3 ? kWaves * 3 * kCodeBytes : 0);
+  static constexpr int kTable = kScales + (kE4M3 ? kWaves * 3 * kScaleBytes : 0);
+  static constexpr int kBytes = kTable + 4 * kTableEntries;
+};
+static_assert(Lds<128, true>::kBytes <= 160 * 1024 && Lds<128, false>::kBytes <= 160 * 1024, "a CU's LDS");
+
+// What V's rows behind a sequence's last one are read as.
+__device__ const u32x4 zero_row[16] = {};
 
 template <typename Tag, int D, bool kE4M3>
-__device__ __forceinline__ void wide_item(const CachedAttnArgs& a, const Item& item, uint16_t* smem) {
+__device__ __forceinline__ void pp_item(const CachedAttnArgs& a, const Item& item, char* smem) {
   using E = Elem<Tag>;
-  constexpr int kTile = kTileElems<D>;
-  // Two slots of K tiles, of V tiles, of rows' offsets (K, V) and of scales (K, V).
-  uint64_t* offsets = reinterpret_cast<uint64_t*>(smem + 4 * kTile);
-  float* scales = reinterpret_cast<float*>(offsets + 4 * kKeys);
-  auto k_lds = [&](int slot) { return smem + slot * kTile; };
-  auto v_lds = [&](int slot) { return smem + (2 + slot) * kTile; };
+  using P = Piece<D, kE4M3>;
+  using L = Lds<D, kE4M3>;
+  constexpr int kStages = kStagesOf<kE4M3>;
+  constexpr int kSlotBytes = L::kSlotBytes;
+  constexpr int kVRingBytes = L::kRingBytes;
+  const char* lds_bytes = smem;
 
   // (Opaque: what follows from it is worked out again for every item instead of being kept, which took 127 more
   // registers than there are.)
@@ -65,238 +78,464 @@ __device__ __forceinline__ void wide_item(const CachedAttnArgs& a, const Item& i
   asm volatile("" : "+v"(tid));
   const int lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int group = wave >> 2;
   const int half = lane >> 5;
 
   const Sequence& seq = item.seq;
   const int rows = seq.count * a.group;
-  const int offset = seq.len - seq.count;  // position of the first new token
-  const int row0 = item.block * kRows + wave * kWaveRows;
+  const int q0 = item.block * kRows;
+  const int row0 = q0 + wave * kWaveRows;
   const int my_row = row0 + (lane & 31);
-  const int my_token = token_of_row(a, my_row);
-  const int my_head = item.hkv * a.group + my_row - my_token * a.group;
-  const bool mine = my_row < rows;
+  const int last = seq.len - 1;
 
-  const int t_begin = item.begin;
-  const int t_end = item.end;
-  const int64_t q_base = a.c.cu_seqlens ? seq.start * a.q_ss : item.b * a.q_bs;
+  // Keys and positions count from the item's first tile.
+  const int num_tiles = item.end - item.begin;
+  const int key0 = item.begin * kKeys;
+  const int offset = seq.len - seq.count - key0;
+  const int seqlen_k = seq.len - key0;
+  // Tiles this wave sees any key of, and the first whose scores need masking.
+  int my_tiles = num_tiles;
+  int mask_from = seqlen_k / kKeys;
+  if (a.causal) {
+    const int end = token_of_row(a, row0 + kWaveRows - 1) + offset;
+    my_tiles = end < 0 ? 0 : min(num_tiles, end / kKeys + 1);
+    const int x = token_of_row(a, row0) + offset - (kKeys - 1);
+    mask_from = min(mask_from, x < 0 ? 0 : x / kKeys + 1);
+  }
+  if (row0 >= rows) my_tiles = 0;
+  const int last_key = a.causal ? min(seqlen_k - 1, token_of_row(a, my_row) + offset) : seqlen_k - 1;
+
   u32x4 qf[D / 16];
   {
-    const uint16_t* src = a.q + q_base + (mine ? my_token : 0) * a.q_ss +
-                          (mine ? my_head : item.hkv * a.group) * a.q_hs + 8 * half;
+    const bool in = my_row < rows;
+    const int token = token_of_row(a, in ? my_row : 0);
+    const int head = item.hkv * a.group + (in ? my_row : 0) - token * a.group;
+    const uint16_t* src = a.q + (a.c.cu_seqlens ? seq.start * a.q_ss : item.b * a.q_bs) + token * a.q_ss +
+                          head * a.q_hs + 8 * half;
 #pragma unroll
-    for (int ks = 0; ks < D / 16; ++ks) qf[ks] = mine ? load16(src + 16 * ks) : u32x4{0, 0, 0, 0};
+    for (int ks = 0; ks < D / 16; ++ks) qf[ks] = in ? load16(src + 16 * ks) : u32x4{0, 0, 0, 0};
   }
 
-  int k_off[D / 16];
+  int k_lds[D / 16];
 #pragma unroll
-  for (int ks = 0; ks < D / 16; ++ks) k_off[ks] = k_lane_offset<D>(ks, lane);
-  int v_off[D / 32][2];
+  for (int ks = 0; ks < D / 16; ++ks) k_lds[ks] = k_lane_offset<D>(ks, lane);
+  // (V offsets are biased by the K ring's size, so that every slot is an immediate.)
+  int v_lds[D / 32][2];
+  int v_bias = kVRingBytes;
+  asm volatile("" : "+v"(v_bias));
 #pragma unroll
   for (int nb = 0; nb < D / 32; ++nb) {
-    v_off[nb][0] = v_lane_offset<D>(nb, 0, lane);
-    v_off[nb][1] = v_lane_offset<D>(nb, 1, lane);
+    v_lds[nb][0] = v_lane_offset<D>(nb, 0, lane) + v_bias;
+    v_lds[nb][1] = v_lane_offset<D>(nb, 1, lane) + v_bias;
   }
 
-  // Tile loads: piece j of a tensor's tile gives this thread 16 bytes of row load_row + j kRowStep. Lane l of
-  // waves 0 to 3 works out where key l's K row, V row, K scale and V scale lie, and leaves the offset, or
-  // the scale itself, in LDS.
-  using P = Piece<D, kE4M3>;
-  constexpr int kRowStep = kThreads / P::kPerRow;
-  constexpr int kPieces = kKeys / kRowStep;
-  const int load_row = tid / P::kPerRow;
-  const int load_col = tid % P::kPerRow * P::kElems;
-  const int last = seq.len - 1;  // rows behind it are not read: it takes their place in K, zeros in V
-  const bool for_v = wave & 1;
-  const bool for_scale = wave >> 1;
-  const RowSpace space = kE4M3 && for_scale ? scales_of(a.c, for_v, item.b, item.hkv)
-                                            : rows_of(a.c, for_v, item.b, item.hkv, P::kElem);
-  const char* kp = rows_of(a.c, false, item.b, item.hkv, P::kElem).base + load_col * P::kElem;
-  const char* vp = rows_of(a.c, true, item.b, item.hkv, P::kElem).base + load_col * P::kElem;
-  struct Pieces {
-    u32x4 k[kPieces], v[kPieces];
+  // The blocks that hold the item's keys, as the table has them (kept in LDS while they fit; a load here would
+  // wait for all tile loads before it).
+  const bool paged = a.c.block_tables != nullptr;
+  const int32_t* table_row = a.c.block_tables + item.b * a.c.block_tables_stride;
+  int* table = reinterpret_cast<int*>(smem + L::kTable);
+  auto block_of = [&](int key) { return a.c.page_shift >= 0 ? key >> a.c.page_shift : key / a.c.rows; };
+  int first_block = 0;
+  bool in_lds = false;
+  if (paged && num_tiles > 0) {
+    first_block = block_of(key0);
+    const int blocks = block_of(min(item.end * kKeys - 1, last)) - first_block + 1;
+    in_lds = blocks <= kTableEntries;
+    if (in_lds) {
+      for (int i = tid; i < blocks; i += kThreads) table[i] = table_row[first_block + i];
+    }
+    __syncthreads();
+  }
+
+  // This wave's 16 rows of its group's tensor in every tile: lane l works out where row l % 16 lies, and
+  // piece j of the lane is 16 bytes of row kRowStep j + l / kPerRow.
+  constexpr int kRowStep = 64 / P::kPerRow;
+  constexpr int kPieces = 16 / kRowStep;
+  constexpr int kLoads = kPieces + (kE4M3 ? 1 : 0);  // of a tile and wave
+  const int tile_row0 = 16 * (wave & 3);
+  const int piece_row = lane / P::kPerRow;
+  const int piece = lane % P::kPerRow;
+  const bool for_v = group == 1;
+  const RowSpace space = rows_of(a.c, for_v, item.b, item.hkv, P::kElem);
+  const RowSpace scale_space = scales_of(a.c, for_v, item.b, item.hkv);
+  const int ring = for_v ? kVRingBytes : 0;
+  // Tile t's pieces go into its ring slot, codes and their scales into places of the wave's own.
+  const int my_codes = L::kCodes + wave * 3 * L::kCodeBytes;
+  const int my_scales = L::kScales + wave * 3 * L::kScaleBytes;
+  const uint32_t lds_base = lds_address(smem);
+  uint64_t row_at = 0;  // address of the lane's row of the tile being asked for
+  // Rows behind the sequence's last one are not read: it takes their place in K, zeros in V.
+  auto locate = [&](int t, int slot) {
+    const int at_key = key0 + t * kKeys + tile_row0 + (lane & 15);
+    const int key = min(at_key, last);
+    cache::Place at{0, key};
+    if (paged) {
+      const int block = block_of(key);
+      // (Past the item's last tile the entry is not used; it is kept within the table's place.)
+      at.outer = in_lds ? table[min(block - first_block, kTableEntries - 1)] : table_row[block];
+      at.row = cache::row_in_block(a.c, key);
+    }
+    row_at = reinterpret_cast<uint64_t>(space.base) + space.offset(a.c, at);
+    if constexpr (kE4M3)
+      global_load_u8_to_lds_asm(scale_space.base + scale_space.offset(a.c, at),
+                                lds_base + my_scales + (static_cast<unsigned>(slot) % 3) * L::kScaleBytes);
+    if (for_v && at_key > last) row_at = reinterpret_cast<uint64_t>(zero_row);
   };
-  auto find = [&](int tile) { return cache::place(a.c, item.b, min(tile * kKeys + lane, last)); };
-  // The offsets of a tile's rows into LDS; the scale waves ask for their bytes.
-  auto locate = [&](int tile, const cache::Place& at, uint32_t& byte) {
-    if (!for_scale) {
-      offsets[((tile & 1) * 2 + wave) * kKeys + lane] = space.offset(a.c, at);
-    } else if constexpr (kE4M3) {
-      byte = static_cast<uint8_t>(space.base[space.offset(a.c, at)]);
-    }
+  auto ask = [&](int slot, int j) {
+    const int from = kRowStep * j + piece_row;
+    const uint32_t lo = __shfl(static_cast<int>(row_at), from);
+    const uint32_t hi = __shfl(static_cast<int>(row_at >> 32), from);
+    // (LDS chunk `piece` of a row of 16-bit elements holds the row's chunk piece ^ swz.)
+    const int chunk = kE4M3 ? piece : piece ^ prefill::swz<D>(tile_row0 + from);
+    const uint32_t to = kE4M3 ? my_codes + (static_cast<unsigned>(slot) % 3) * L::kCodeBytes
+                              : ring + tile_row0 * 2 * D + (static_cast<unsigned>(slot) % kStages) * kSlotBytes;
+    global_load16_to_lds_asm(reinterpret_cast<const char*>(static_cast<uint64_t>(hi) << 32 | lo) + 16 * chunk,
+                             lds_base + to + 1024 * j);
   };
-  auto put_scales = [&](int tile, uint32_t byte) {
-    if constexpr (kE4M3) {
-      if (for_scale) scales[((tile & 1) * 2 + for_v) * kKeys + lane] = cache::scale_of(byte);
-    }
+  // Codes: a piece of a tile's, with its row's scale, becomes two 16-byte stores.
+  constexpr int kPuts = kE4M3 ? 2 * kPieces : 0;
+  u32x4 code{};
+  float scale = 0.f;
+  auto take = [&](int slot, int j) {
+    const unsigned s = static_cast<unsigned>(slot) % 3;
+    code = *reinterpret_cast<const u32x4*>(smem + my_codes + s * L::kCodeBytes + 1024 * j + 16 * lane);
+    scale = cache::scale_of(
+        *reinterpret_cast<const uint32_t*>(smem + my_scales + s * L::kScaleBytes + 4 * (kRowStep * j + piece_row)));
   };
-  auto load = [&](int tile, Pieces& r) {
-    const uint64_t* at = offsets + (tile & 1) * 2 * kKeys + load_row;
-#pragma unroll
-    for (int j = 0; j < kPieces; ++j) {
-      r.k[j] = load16(kp + at[j * kRowStep]);
-      r.v[j] = load16(vp + at[kKeys + j * kRowStep]);
-    }
-  };
-  auto store = [&](int tile, Pieces& r) {
-    if (tile * kKeys + kKeys - 1 > last) {
-#pragma unroll
-      for (int j = 0; j < kPieces; ++j)
-        if (tile * kKeys + load_row + j * kRowStep > last) r.v[j] = u32x4{0, 0, 0, 0};
-    }
-    const float* sc = scales + (tile & 1) * 2 * kKeys + load_row;
-#pragma unroll
-    for (int j = 0; j < kPieces; ++j) {
-      const int row = load_row + j * kRowStep;
-      put_piece<Tag, D, kE4M3>(k_lds(tile & 1), row, load_col, r.k[j], kE4M3 ? sc[j * kRowStep] : 0.f);
-      put_piece<Tag, D, kE4M3>(v_lds(tile & 1), row, load_col, r.v[j], kE4M3 ? sc[kKeys + j * kRowStep] : 0.f);
-    }
+  auto put = [&](int slot, int i) {
+    const int row = tile_row0 + kRowStep * (i / 2) + piece_row;
+    uint16_t* tile = reinterpret_cast<uint16_t*>(smem + ring + (static_cast<unsigned>(slot) % kStages) * kSlotBytes);
+    const u32x2 lo = cache::values4<Tag>(code[2 * (i % 2)], scale);
+    const u32x2 hi = cache::values4<Tag>(code[2 * (i % 2) + 1], scale);
+    *reinterpret_cast<u32x4*>(tile + tile_offset<D>(row, 16 * piece + 8 * (i % 2))) = u32x4{lo[0], lo[1], hi[0], hi[1]};
   };
 
   f32x16 o[D / 32];
 #pragma unroll
   for (int nb = 0; nb < D / 32; ++nb) o[nb] = f32x16{};
-  float ref = -INFINITY;  // reference point of o and l, log2 units; -inf until a key is seen
+  f32x16 s0 = f32x16{};
+  f32x16 s1 = f32x16{};
+  u32x4 pf[4] = {};
+  float ref = kNoRef;
   float l = 0.f;
   const float sl2 = a.scale_log2;
-  // Last key that this lane's row, the wave's first and the wave's last row see.
-  const int last_key = a.causal ? min(last, my_token + offset) : last;
-  const int first_limit = a.causal ? min(last, token_of_row(a, row0) + offset) : last;
-  const int wave_limit = row0 >= rows ? -1 : a.causal ? min(last, token_of_row(a, row0 + kWaveRows - 1) + offset) : last;
 
-  auto tile_step = [&](int t, int slot) {
-    const int k0 = t * kKeys;
-    if (k0 > wave_limit) return;
-    const char* kt = reinterpret_cast<const char*>(k_lds(slot));
-    const char* vt = reinterpret_cast<const char*>(v_lds(slot));
-    f32x16 s0 = f32x16{};
-    f32x16 s1 = f32x16{};
-#pragma unroll
-    for (int ks = 0; ks < D / 16; ++ks) {
-      s0 = E::mfma32(prefill::lds_load16(kt, k_off[ks]), qf[ks], s0);
-      s1 = E::mfma32(prefill::lds_load16(kt + kKeyBlockBytes<D>, k_off[ks]), qf[ks], s1);
+  // The MFMA phase of a period (prefill_pp.hip): P V of the tile before, K Q^T of this one, 12 P V steps
+  // first, the row max of the new scores between the last 4.
+  constexpr int kPv = 4 * (D / 32);
+  constexpr int kQk = 2 * (D / 16);
+  constexpr int kSteps = kPv + kQk;
+  constexpr int kTail = 4;
+  constexpr int kLeadPv = kPv - kTail;
+  auto step_at = [](auto n_tag, auto full_tag) constexpr {
+    constexpr int n = decltype(n_tag)::value;
+    if constexpr (!decltype(full_tag)::value) {
+      return n;
+    } else {
+      return n < kLeadPv ? n : n < kLeadPv + kQk ? kPv + (n - kLeadPv) : n - kQk;
     }
-    // (K fragments two steps ahead of their MFMAs: prefill_fwd.hip)
-    __builtin_amdgcn_sched_group_barrier(0x100, 4, 1);
-#pragma unroll
-    for (int ks = 0; ks < D / 16 - 2; ++ks) {
-      __builtin_amdgcn_sched_group_barrier(0x008, 2, 1);
-      __builtin_amdgcn_sched_group_barrier(0x100, 2, 1);
+  };
+  auto read_frag = [&](int slot, auto i_tag) -> u32x4 {
+    constexpr int i = decltype(i_tag)::value;
+    if constexpr (i < kPv) {
+      constexpr int kk = i / (D / 32), nb = i % (D / 32);
+      const char* vt = lds_bytes + (static_cast<unsigned>(slot + kStages - 1) % kStages) * kSlotBytes;
+      return v_frag_at(vt + kk * kKeyStepBytes<D>, v_lds[nb][0], v_lds[nb][1]);
+    } else {
+      constexpr int j = i - kPv, ks = j / 2, blk = j % 2;
+      const char* kt = lds_bytes + (static_cast<unsigned>(slot) % kStages) * kSlotBytes;
+      return prefill::lds_load16(kt + blk * kKeyBlockBytes<D>, k_lds[ks]);
     }
-    __builtin_amdgcn_sched_group_barrier(0x008, 4, 1);
-    if (k0 + kKeys - 1 > first_limit) {
-      const int lim = last_key - k0 - 4 * half;
+  };
+  u32x4 pre[kAhead];
+  auto prefetch = [&](int slot) {
+    static_for<0, kAhead>([&](auto i) { pre[decltype(i)::value] = read_frag(slot, i); });
+  };
+  auto prefetch_qk = [&](int slot) {
+    static_for<0, kAhead>([&](auto i) {
+      pre[decltype(i)::value] = read_frag(slot, std::integral_constant<int, kPv + decltype(i)::value>{});
+    });
+  };
+  float tile_mx = kNoRef;
+  float mx_t[10], mx_u[4], mx_w = 0.f;
+  auto max_op = [&](auto k_tag) {
+    constexpr int k = decltype(k_tag)::value;
+    if constexpr (k < 5) {
+      mx_t[k] = max3_f32(s0[3 * k], s0[3 * k + 1], s0[3 * k + 2]);
+    } else if constexpr (k < 10) {
+      mx_t[k] = max3_f32(s1[3 * (k - 5)], s1[3 * (k - 5) + 1], s1[3 * (k - 5) + 2]);
+    } else if constexpr (k < 13) {
+      mx_u[k - 10] = max3_f32(mx_t[3 * (k - 10)], mx_t[3 * (k - 10) + 1], mx_t[3 * (k - 10) + 2]);
+    } else if constexpr (k == 13) {
+      mx_u[3] = max3_f32(mx_t[9], s0[15], s1[15]);
+    } else if constexpr (k == 14) {
+      mx_w = max3_f32(mx_u[0], mx_u[1], mx_u[2]);
+    } else if constexpr (k == 15) {
+      mx_w = max2_f32(mx_w, mx_u[3]);
+    } else if constexpr (k == 16) {
+      mx_w = max_halves(mx_w);
+    } else {
+      tile_mx = mx_w * sl2;
+    }
+  };
+  constexpr int kMaxOps = 18;
+  auto mfma_phase = [&](int slot, auto pv_tag, auto qk_tag, auto&& hook) {
+    constexpr bool kDoPv = decltype(pv_tag)::value;
+    constexpr bool kDoQk = decltype(qk_tag)::value;
+    constexpr bool kFull = kDoPv && kDoQk;
+    constexpr int kFirstLive = kDoPv ? 0 : kPv;
+    constexpr int kEndLive = kDoQk ? kSteps : kPv;
+    u32x4 fr[kSteps];
+    static_for<0, kAhead>([&](auto i) {
+      constexpr int n = kFirstLive + decltype(i)::value;
+      fr[step_at(std::integral_constant<int, n>{}, std::bool_constant<kFull>{})] = pre[decltype(i)::value];
+    });
+    __builtin_amdgcn_s_setprio(1);
+    __builtin_amdgcn_sched_barrier(0);
+    static_for<0, kSteps>([&](auto n_tag) {
+      constexpr int n = decltype(n_tag)::value;
+      constexpr int i = step_at(n_tag, std::bool_constant<kFull>{});
+      if constexpr (n >= kFirstLive && n < kEndLive) {
+        if constexpr (i < kPv) {
+          constexpr int kk = i / (D / 32), nb = i % (D / 32);
+          o[nb] = E::mfma32(fr[i], pf[kk], o[nb]);
+        } else {
+          constexpr int j = i - kPv, ks = j / 2, blk = j % 2;
+          f32x16& acc = blk == 0 ? s0 : s1;
+          acc = E::mfma32(fr[i], qf[ks], ks == 0 ? f32x16{} : acc);
+        }
+      }
+      constexpr int nx = n + kAhead;
+      if constexpr (nx >= kFirstLive + kAhead && nx < kEndLive) {
+        constexpr int ix = step_at(std::integral_constant<int, nx>{}, std::bool_constant<kFull>{});
+        fr[ix] = read_frag(slot, std::integral_constant<int, ix>{});
+      }
+      hook(n_tag);
+      if constexpr (kFull && n >= kLeadPv + kQk) {
+        constexpr int k = n - (kLeadPv + kQk);
+        static_for<k * kMaxOps / kTail, (k + 1) * kMaxOps / kTail>([&](auto op) { max_op(op); });
+      }
+      __builtin_amdgcn_sched_barrier(0);
+    });
+    __builtin_amdgcn_s_setprio(0);
+    if constexpr (kDoQk && !kDoPv) static_for<0, kMaxOps>([&](auto op) { max_op(op); });
+  };
+
+  auto softmax_phase = [&](int t) {
+    float mx = tile_mx;
+    if (t >= mask_from) {
+      asm volatile("" ::: "memory");
+      const int lim = last_key - t * kKeys - 4 * half;
 #pragma unroll
       for (int j = 0; j < 16; ++j) {
         const int kj = acc_key(j, 0);
-        if (kj > lim) s0[j] = -INFINITY;
-        if (kj + 32 > lim) s1[j] = -INFINITY;
+        s0[j] = kj > lim ? -INFINITY : s0[j];
+        s1[j] = kj + 32 > lim ? -INFINITY : s1[j];
+        __builtin_amdgcn_sched_barrier(0);  // (one compare and one select at a time: prefill_pp.hip)
       }
+      mx = max_halves(max_of(s0, s1)) * sl2;
     }
-    // The reference point moves to the row's running max when that has grown by more than kMoveSlack over
-    // it (prefill_tile.hpp).
-    const float top = max_halves(max_of(s0, s1)) * sl2;
-    const bool move = top > ref + kMoveSlack;
-    if (wave_any(move)) {
-      const float alpha = move ? exp2_fast(ref - top) : 1.f;  // ref = -inf gives 0
-      ref = move ? top : ref;
-      l *= alpha;
+    if (wave_any(mx > ref + kMoveSlack)) {
+      asm volatile("" ::: "memory");
+      const float moved = max2_f32(ref, mx);
+      const float alpha = exp2_fast(ref - moved);  // 0 for a row's first key
+      ref = moved;
 #pragma unroll
       for (int nb = 0; nb < D / 32; ++nb) o[nb] *= alpha;
+      l *= alpha;
     }
-    const float shift = ref == -INFINITY ? 0.f : ref;
-    float r0 = 0.f;
-    float r1 = 0.f;
+    f32x16 p0, p1;
 #pragma unroll
     for (int j = 0; j < 16; ++j) {
-      s0[j] = exp2_fast(fmaf(s0[j], sl2, -shift));
-      r0 += s0[j];
-      s1[j] = exp2_fast(fmaf(s1[j], sl2, -shift));
-      r1 += s1[j];
+      p0[j] = exp2_fast(fmaf(s0[j], sl2, -ref));
+      p1[j] = exp2_fast(fmaf(s1[j], sl2, -ref));
     }
+    float r0 = p0[0];
+    float r1 = p1[0];
+#pragma unroll
+    for (int j = 1; j < 16; ++j) {
+      r0 += p0[j];
+      r1 += p1[j];
+    }
+    pf[0] = p_frag<Tag, 0>(p0);
+    pf[1] = p_frag<Tag, 1>(p0);
+    pf[2] = p_frag<Tag, 0>(p1);
+    pf[3] = p_frag<Tag, 1>(p1);
     l += r0 + r1;
-    const u32x4 pf[4] = {p_frag<Tag, 0>(s0), p_frag<Tag, 1>(s0), p_frag<Tag, 0>(s1), p_frag<Tag, 1>(s1)};
-#pragma unroll
-    for (int kk = 0; kk < 4; ++kk) {
-#pragma unroll
-      for (int nb = 0; nb < D / 32; ++nb)
-        o[nb] = E::mfma32(v_frag_at(vt + kk * kKeyStepBytes<D>, v_off[nb][0], v_off[nb][1]), pf[kk], o[nb]);
-    }
   };
 
-  if (t_begin < t_end) {
-    // Iteration t multiplies tile t. Before it, tile t + 1's pieces go into the other slot, tile t + 2's are
-    // asked for, tile t + 3's rows are located and tile t + 4's table entries are asked for; scales run one
-    // iteration behind the offsets. Tiles past the end repeat the last row and are not used.
-    Pieces in;
-    uint32_t byte = 0;
-    cache::Place at = find(t_begin);
-    locate(t_begin, at, byte);
-    put_scales(t_begin, byte);
-    at = find(t_begin + 1);
-    locate(t_begin + 1, at, byte);
-    put_scales(t_begin + 1, byte);
-    __syncthreads();
-    load(t_begin, in);
-    at = find(t_begin + 2);
-    store(t_begin, in);
-    load(t_begin + 1, in);
-    __syncthreads();
-    locate(t_begin + 2, at, byte);
-    at = find(t_begin + 3);
-    __syncthreads();
-    for (int t = t_begin; t < t_end; ++t) {
-      store(t + 1, in);
-      load(t + 2, in);
-      put_scales(t + 2, byte);
-      locate(t + 3, at, byte);
-      at = find(t + 4);
-      tile_step(t, t & 1);
-      phase_barrier();  // (the loads in flight need not have come back)
+  // Tiles that loads run ahead: in the tokens' type V's ring has no place for a third.
+  constexpr auto kLeadOf = [](int g) { return kE4M3 || g == 0 ? 3 : 2; };
+  using kFirstT = std::integral_constant<int, 0>;
+  using kFullT = std::integral_constant<int, 1>;
+  using kLastT = std::integral_constant<int, 2>;
+  using kLoadsT = std::integral_constant<int, 3>;
+  auto run = [&](auto group_tag) {
+    constexpr int kGroup = decltype(group_tag)::value;
+    constexpr int kLead = kLeadOf(kGroup);
+    auto period = [&](int m, int slot, auto mode_tag) {
+      constexpr int kMode = decltype(mode_tag)::value;
+      constexpr bool kDoPv = kMode == kFullT::value || kMode == kLastT::value;
+      constexpr bool kDoQk = kMode == kFirstT::value || kMode == kFullT::value;
+      auto hook = [&](auto i_tag) {
+        constexpr int i = decltype(i_tag)::value;
+        // (Codes of tile m + 1 have landed, tile m + 2's are on their way.)
+        if constexpr (kE4M3 && i == 0) prefill::pp::wait_vmcnt<kLoads>();
+        if constexpr (i % 6 == 0 && i / 3 < kPuts) take(slot + 1, i / 6);
+        if constexpr (i % 3 == 2 && i / 3 < kPuts) put(slot + 1, i / 3);
+        constexpr int kAskFrom = 3 * kPuts + 1;
+        if constexpr (i == kAskFrom) locate(m + kLead, slot + kLead);
+        constexpr int k = i - kAskFrom - 2;
+        if constexpr (k >= 0 && k % 3 == 0 && k / 3 < kPieces) ask(slot + kLead, k / 3);
+        static_assert(kAskFrom + 2 + 3 * (kPieces - 1) < kSteps, "the tile's moves fit the phase");
+      };
+      auto mfma = [&]() {
+        if constexpr (kMode == kLoadsT::value) {
+          static_for<0, kSteps>([&](auto i) { hook(i); });
+        } else {
+          mfma_phase(slot, std::bool_constant<kDoPv>{}, std::bool_constant<kDoQk>{}, hook);
+        }
+      };
+      if constexpr (kGroup == 0) {
+        if constexpr (kMode == kFirstT::value) prefetch_qk(slot);
+        mfma();
+        if constexpr (kDoQk) {
+          prefetch(slot + 1);
+          softmax_phase(m);
+        }
+      } else {
+        if constexpr (kMode == kFirstT::value) prefetch_qk(slot);
+        if constexpr (kDoPv) {
+          prefetch(slot);
+          softmax_phase(m - 1);
+        }
+        mfma();
+      }
+      // In the tokens' type: tile m + 1's loads into LDS have landed, later ones are on their way; the barrier
+      // publishes it.
+      if constexpr (!kE4M3) prefill::pp::wait_vmcnt<(kLead - 1) * kLoads>();
+      phase_barrier();
+    };
+    int m = 0;
+    if (my_tiles > 0) {
+      period(0, 0, kFirstT{});
+      for (m = 1; m < my_tiles;) {
+        bool done = false;
+        static_for<0, kStages>([&](auto j) {
+          if (done) return;
+          period(m, (1 + decltype(j)::value) % kStages, kFullT{});
+          done = ++m == my_tiles;
+        });
+      }
+      period(m, m % kStages, kLastT{});
+      ++m;
+    }
+    for (; m <= num_tiles; ++m) period(m, m % kStages, kLoadsT{});
+  };
+  if (num_tiles > 0) {
+    auto ask_tile = [&](int i) {
+      locate(i, i);
+      static_for<0, kPieces>([&](auto j) { ask(i, decltype(j)::value); });
+    };
+    ask_tile(0);
+    ask_tile(1);
+    if (kE4M3 || group == 0) ask_tile(2);
+    if constexpr (kE4M3) {
+      prefill::pp::wait_vmcnt<2 * kLoads>();
+      static_for<0, kPuts>([&](auto i) {
+        if constexpr (decltype(i)::value % 2 == 0) take(0, decltype(i)::value / 2);
+        put(0, decltype(i)::value);
+      });
+    } else if (group == 0) {
+      prefill::pp::wait_vmcnt<2 * kLoads>();
+    } else {
+      prefill::pp::wait_vmcnt<kLoads>();
+    }
+    phase_barrier();
+    if (group == 0) {
+      run(std::integral_constant<int, 0>{});
+    } else {
+      run(std::integral_constant<int, 1>{});
     }
   }
 
+  prefill::pp::wait_vmcnt<0>();  // (the loads of tiles past the end have landed before LDS is used again)
+  phase_barrier();
+  // Rows leave whole: each wave stages its 32 in its own part of the (free) rings, padded by 16 bytes.
   const float lt = sum_halves(l);
+    constexpr int kStageRow = 4 * D + 16;
+  static_assert(kWaves * 16 * kStageRow <= L::kBytes, "16 rows of each wave fit");
+  char* stage = smem + wave * 16 * kStageRow;
+  const float inv = inverse(lt);
   if (item.partial) {
-    if (mine) {
-      const int64_t slot_row = a.wide_partials + static_cast<int64_t>(item.slot) * kRows + wave * kWaveRows + (lane & 31);
-      float* po = a.partial_o + slot_row * D + 4 * half;
+    // (In two halves of 16 rows.)
+    float* po = a.partial_o + (a.wide_partials + static_cast<int64_t>(item.slot) * kRows + wave * kWaveRows) * D;
 #pragma unroll
-      for (int nb = 0; nb < D / 32; ++nb) {
+    for (int part = 0; part < 2; ++part) {
+      if (((lane >> 4) & 1) == part) {
+        char* w = stage + (lane & 15) * kStageRow + 16 * half;
 #pragma unroll
-        for (int g = 0; g < 4; ++g)
-          *reinterpret_cast<f32x4*>(po + 32 * nb + 8 * g) =
-              f32x4{o[nb][4 * g], o[nb][4 * g + 1], o[nb][4 * g + 2], o[nb][4 * g + 3]};
+        for (int nb = 0; nb < D / 32; ++nb) {
+#pragma unroll
+          for (int g = 0; g < 4; ++g)
+            *reinterpret_cast<f32x4*>(w + 32 * (4 * nb + g)) =
+                f32x4{o[nb][4 * g], o[nb][4 * g + 1], o[nb][4 * g + 2], o[nb][4 * g + 3]};
+        }
       }
-      if (half == 0) a.partial_ml[slot_row] = point_and_sum(ref, lt);
+      constexpr int kLanes = D / 4;  // of a row
+      const int c = lane % kLanes;
+#pragma unroll
+      for (int j = 0; j < 16 * kLanes / 64; ++j) {
+        const int r = j * (64 / kLanes) + lane / kLanes;
+        const f32x4 x = *reinterpret_cast<const f32x4*>(stage + r * kStageRow + 16 * c);
+        if (row0 + 16 * part + r < rows) *reinterpret_cast<f32x4*>(po + (16 * part + r) * D + 4 * c) = x;
+      }
     }
+    if (my_row < rows && half == 0)
+      a.partial_ml[a.wide_partials + static_cast<int64_t>(item.slot) * kRows + my_row - q0] = point_and_sum(ref, lt);
     return;
   }
-  if (!mine) return;
-  const float inv = inverse(lt);
-  const int64_t o_base = a.c.cu_seqlens ? seq.start * a.o_ss : item.b * a.o_bs;
-  uint16_t* orow = a.o + o_base + my_token * a.o_ss + my_head * a.o_hs;
+  constexpr int kOutRow = 2 * D + 16;
+  stage = smem + wave * kWaveRows * kOutRow;
+  {
+    char* w = stage + (lane & 31) * kOutRow + 8 * half;
 #pragma unroll
-  for (int nb = 0; nb < D / 32; ++nb) {
+    for (int nb = 0; nb < D / 32; ++nb) {
 #pragma unroll
-    for (int g = 0; g < 4; ++g)
-      *reinterpret_cast<u32x2*>(orow + 32 * nb + 8 * g + 4 * half) =
-          u32x2{E::pack2(o[nb][4 * g] * inv, o[nb][4 * g + 1] * inv),
-                E::pack2(o[nb][4 * g + 2] * inv, o[nb][4 * g + 3] * inv)};
+      for (int g = 0; g < 4; ++g)
+        *reinterpret_cast<u32x2*>(w + 16 * (4 * nb + g)) =
+            u32x2{E::pack2(o[nb][4 * g] * inv, o[nb][4 * g + 1] * inv),
+                  E::pack2(o[nb][4 * g + 2] * inv, o[nb][4 * g + 3] * inv)};
+    }
   }
-  if (half == 0)
-    a.lse[(static_cast<int64_t>(seq.start) + my_token) * a.heads + my_head] =
+  constexpr int kLanes = D / 8;  // of a row
+  uint16_t* out = a.o + (a.c.cu_seqlens ? seq.start * a.o_ss : item.b * a.o_bs) + 8 * (lane % kLanes);
+#pragma unroll
+  for (int j = 0; j < kWaveRows * kLanes / 64; ++j) {
+    const int r = j * (64 / kLanes) + lane / kLanes;
+    const u32x4 x = *reinterpret_cast<const u32x4*>(stage + r * kOutRow + 16 * (lane % kLanes));
+    if (row0 + r < rows) {
+      const int token = token_of_row(a, row0 + r);
+      const int head = item.hkv * a.group + row0 + r - token * a.group;
+      *reinterpret_cast<u32x4*>(out + token * a.o_ss + head * a.o_hs) = x;
+    }
+  }
+  if (my_row < rows && half == 0) {
+    const int token = token_of_row(a, my_row);
+    a.lse[(static_cast<int64_t>(seq.start) + token) * a.heads + item.hkv * a.group + my_row - token * a.group] =
         log_sum(ref, lt);
+  }
 }
 
 template <typename Tag, int D, bool kE4M3>
 __global__ void __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2, 2)))
     cached_wide_kernel(const CachedAttnArgs a) {
-  __shared__ __attribute__((aligned(16))) uint16_t smem[4 * kTileElems<D> + 4 * kKeys * (8 + 4) / 2];
+  __shared__ __attribute__((aligned(16))) char smem[Lds<D, kE4M3>::kBytes];
   Segments<kWide, D> segments(a);
   Item item;
   while (segments.next(a, item)) {
-    wide_item<Tag, D, kE4M3>(a, uniform(item), smem);
-    __syncthreads();  // (the next item uses the LDS again)
+    pp_item<Tag, D, kE4M3>(a, uniform(item), smem);
+    phase_barrier();  // (the next item uses the LDS again)
   }
 }
 
@@ -317,9 +556,12 @@ hipError_t launch_typed(const CachedAttnArgs& args, int64_t workgroups, bool e4m
 hipError_t launch_cached_wide(const CachedAttnArgs& args, int64_t workgroups, DType dtype, bool e4m3, int head_dim,
                               hipStream_t stream) {
   using namespace cached;
-  if (head_dim == 128) return launch_cached_pp(args, workgroups, dtype, e4m3, stream);
-  return dtype == DType::bf16 ? launch_typed<bf16_tag, 64>(args, workgroups, e4m3, stream)
-                              : launch_typed<f16_tag, 64>(args, workgroups, e4m3, stream);
+  if (dtype == DType::bf16) {
+    return head_dim == 64 ? launch_typed<bf16_tag, 64>(args, workgroups, e4m3, stream)
+                          : launch_typed<bf16_tag, 128>(args, workgroups, e4m3, stream);
+  }
+  return head_dim == 64 ? launch_typed<f16_tag, 64>(args, workgroups, e4m3, stream)
+                        : launch_typed<f16_tag, 128>(args, workgroups, e4m3, stream);
 }
 
 }  // namespace fl

@@ -153,6 +153,11 @@ __device__ __forceinline__ void global_load16_to_lds_asm(const void* p, uint32_t
   const uint32_t m0 = static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<int>(lds_addr)));
   asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" : : "v"(p), "s"(m0) : "memory", "m0");
 }
+// A byte per lane: lane l's, zero-extended, goes to the dword at lds_addr + 4 l.
+__device__ __forceinline__ void global_load_u8_to_lds_asm(const void* p, uint32_t lds_addr) {
+  const uint32_t m0 = static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<int>(lds_addr)));
+  asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_ubyte %0, off" : : "v"(p), "s"(m0) : "memory", "m0");
+}
 // 32-bit LDS address of a __shared__ object.
 __device__ __forceinline__ uint32_t lds_address(const void* p) {
   typedef __attribute__((address_space(3))) const void lds_cvoid;

@@ -241,12 +241,10 @@ struct CachedPlan {
 CachedPlan plan_cached_attn(const CachedAttnArgs& args, int head_dim, bool e4m3, int cu_count);
 hipError_t launch_cached_attn(const CachedAttnArgs& args, const CachedPlan& plan, DType dtype, bool e4m3,
                               int head_dim, hipStream_t stream);
-// Its kernels (cached_narrow.hip; cached_wide.hip, which passes head_dim 128 on to cached_pp.hip), and how many workgroups of the first a CU holds.
+// Its kernels (cached_narrow.hip, cached_wide.hip), and how many workgroups of the first a CU holds.
 int cached_narrow_resident(int head_dim, bool e4m3, int most_rows);
 hipError_t launch_cached_narrow(const CachedAttnArgs& args, const CachedPlan& plan, DType dtype, bool e4m3,
                                 int head_dim, hipStream_t stream);
-hipError_t launch_cached_pp(const CachedAttnArgs& args, int64_t workgroups, DType dtype, bool e4m3,
-                            hipStream_t stream);
 hipError_t launch_cached_wide(const CachedAttnArgs& args, int64_t workgroups, DType dtype, bool e4m3, int head_dim,
                               hipStream_t stream);
 
