@@ -33,23 +33,61 @@ constexpr float kLn2 = 0.693147180559945309f;
 // Running max before the first key: finite, so that a masked score (-inf) gives p = 0.
 constexpr float kNoRef = -1e30f;
 
+// The kernel's arguments (its only parameter), for the compiler to load again from here on: kept in scalar registers
+// from the kernel's start, with what follows from them, a hundred and more were spilled.
+__device__ __forceinline__ const CachedAttnArgs& reload_args() {
+  typedef const CachedAttnArgs __attribute__((address_space(4))) ConstantArgs;
+  ConstantArgs* p = (ConstantArgs*)(__builtin_amdgcn_kernarg_segment_ptr());
+  asm volatile("" : "+s"(p));
+  return *(const CachedAttnArgs*)(p);
+}
+
 __device__ __forceinline__ int token_of_row(const CachedAttnArgs& a, int row) {
   return static_cast<int>((static_cast<uint64_t>(static_cast<uint32_t>(row)) * a.group_mul) >> a.group_shift);
 }
 
 __device__ __forceinline__ int wave_sum(int x) { return __builtin_amdgcn_readlane(wave_inclusive_sum(x), 63); }
+// (The steps of wave_inclusive_sum: a tree of lane permutes through LDS took 0.25 us.)
 __device__ __forceinline__ float wave_sum(float x) {
-#pragma unroll
-  for (int m = 32; m >= 1; m /= 2) x += __shfl_xor(x, m);
-  return x;
+  auto step = [&](auto ctrl, auto rows) {
+    const int from = __builtin_amdgcn_update_dpp(0, __float_as_int(x), decltype(ctrl)::value, decltype(rows)::value, 0xf, false);
+    x += __int_as_float(from);
+  };
+  using std::integral_constant;
+  step(integral_constant<int, 0x111>{}, integral_constant<int, 0xf>{});
+  step(integral_constant<int, 0x112>{}, integral_constant<int, 0xf>{});
+  step(integral_constant<int, 0x114>{}, integral_constant<int, 0xf>{});
+  step(integral_constant<int, 0x118>{}, integral_constant<int, 0xf>{});
+  step(integral_constant<int, 0x142>{}, integral_constant<int, 0xa>{});
+  step(integral_constant<int, 0x143>{}, integral_constant<int, 0xc>{});
+  return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(x), 63));
 }
 
-// Sums over the sequences of a batch: lane l holds sequence 64 i + l of chunk i; chunks behind the first are
-// read again in every pass.
+// n / c for 0 <= n < 2^31 - c and 1 <= c, by a reciprocal: the first quotient is off by at most 1 + n 2^-21 / c, so
+// what it leaves is below c + n 2^-21 in magnitude, whose quotient brings it to one off. (The integer division is some
+// forty instructions on the way to a workgroup's first load.)
+struct Quotient {
+  int c;
+  float r;
+  __device__ __forceinline__ explicit Quotient(int divisor)
+      : c(divisor), r(__builtin_amdgcn_rcpf(static_cast<float>(divisor))) {}
+  __device__ __forceinline__ int of(int n) const {
+    auto left_of = [&](int q) { return static_cast<int>(static_cast<uint32_t>(n) - static_cast<uint32_t>(q) * c); };
+    int q = static_cast<int>(static_cast<float>(n) * r);
+    q += static_cast<int>(static_cast<float>(left_of(q)) * r);
+    const int left = left_of(q);
+    return q + (left >= c ? 1 : 0) - (left < 0 ? 1 : 0);
+  }
+  __device__ __forceinline__ int ceil_of(int n) const { return of(n + c - 1); }
+};
+
+// The sequences of a batch: lane l holds sequence 64 i + l of chunk i; chunks behind the first are read again
+// in every pass.
 struct Batch {
   const CachedAttnArgs& a;
   Sequence first;
-  __device__ __forceinline__ explicit Batch(const CachedAttnArgs& args) : a(args), first(at(__lane_id())) {}
+  __device__ __forceinline__ explicit Batch(const CachedAttnArgs& args) : a(args) { read(); }
+  __device__ __forceinline__ void read() { first = at(__lane_id()); }
   __device__ __forceinline__ Sequence at(int b) const {
     Sequence s{0, 0, 0};
     if (b < a.c.batch) s = cache::sequence(a.c, b);
@@ -57,16 +95,17 @@ struct Batch {
   }
   __device__ __forceinline__ Sequence lane_of(int base) const { return base == 0 ? first : at(base + __lane_id()); }
   template <typename F>
-  __device__ __forceinline__ auto sum(F f) const {
-    auto total = f(first);
-    for (int base = 64; base < a.c.batch; base += 64) total += f(at(base + __lane_id()));
-    return wave_sum(total);
+  __device__ __forceinline__ void each(F f) const {
+    f(first);
+    for (int base = 64; base < a.c.batch; base += 64) f(at(base + __lane_id()));
   }
   // Sequences that overlap (cu_seqlens does not ascend) could have more items than the grid and the
   // workspace are made for: no item is run then.
   __device__ __forceinline__ bool sound() const {
-    return a.c.cu_seqlens == nullptr ||
-           sum([](const Sequence& s) { return static_cast<float>(s.count); }) <= 1.001f * a.c.tokens;
+    if (a.c.cu_seqlens == nullptr) return true;
+    bool back = false;
+    for (int b = __lane_id(); b < a.c.batch; b += 64) back |= a.c.cu_seqlens[b + 1] < a.c.cu_seqlens[b];
+    return !wave_any(back);
   }
 };
 
@@ -115,16 +154,14 @@ __device__ __forceinline__ void leave(const CachedAttnArgs& a, const Item& item,
 // Items of equal shares: sequence b has blocks_b splits_b H_kv of them, with splits_b = ceil(tiles_b / share).
 // The least share for which no more than `slots` items result (which run at once), 0 if there are more blocks.
 template <Kind kKind, int D>
-__device__ __forceinline__ int even_share(const CachedAttnArgs& a, const Batch& batch, int blocks, int slots) {
+__device__ __forceinline__ int even_share(const CachedAttnArgs& a, const Batch& batch, int blocks, float work, int slots) {
   if (blocks > slots) return 0;
   auto items = [&](int t) {
-    return a.c.heads_kv * batch.sum([&](const Sequence& s) {
-      return blocks_of<kKind, D>(a, s) * max((tiles_of(s) + t - 1) / t, 1);
-    });
+    const Quotient by(t);
+    int total = 0;
+    batch.each([&](const Sequence& s) { total += blocks_of<kKind, D>(a, s) * max(by.ceil_of(tiles_of(s)), 1); });
+    return a.c.heads_kv * wave_sum(total);
   };
-  const float work = a.c.heads_kv * batch.sum([&](const Sequence& s) {
-    return static_cast<float>(blocks_of<kKind, D>(a, s)) * static_cast<float>(tiles_of(s));
-  });
   // sum of ceil(x / t) is at most work / t + blocks.
   int low = max(a.min_tiles, static_cast<int>(work / slots));
   int high = blocks < slots ? max(low, static_cast<int>(work / (slots - blocks) * 1.001f) + 1) : 1 << 28;
@@ -151,7 +188,7 @@ __device__ __forceinline__ bool find_item(const CachedAttnArgs& a, const Batch& 
     const int lane = __lane_id();
     const Sequence s = batch.lane_of(base);
     const int tiles = tiles_of(s);
-    const int splits = a.num_splits > 0 ? a.num_splits : share > 0 ? max((tiles + share - 1) / share, 1) : 1;
+    const int splits = a.num_splits > 0 ? a.num_splits : share > 0 ? max(Quotient(share).ceil_of(tiles), 1) : 1;
     const int items = blocks_of<kKind, D>(a, s) * splits * a.c.heads_kv;
     const int slots = splits > 1 ? items : 0;
     const int all = wave_inclusive_sum(items);
@@ -159,7 +196,7 @@ __device__ __forceinline__ bool find_item(const CachedAttnArgs& a, const Batch& 
     int from = all - items;  // items and slots of the chunk before the lane's
     int from_slot = all_slots - slots;
     if (sorted) {
-      const int length = tiles / splits;
+      const int length = Quotient(splits).of(tiles);
       from = from_slot = 0;
       const int here = min(a.c.batch - base, 64);
       for (int j = 0; j < here; ++j) {
@@ -179,14 +216,18 @@ __device__ __forceinline__ bool find_item(const CachedAttnArgs& a, const Batch& 
       const int n = of_owner(splits);
       const int at = of_owner(local);
       const int units = a.c.heads_kv * n;  // items of a block
-      const int turn = at / units;
+      const int turn = Quotient(units).of(at);
       const int unit = at - turn * units;
-      item.hkv = unit / n;
+      const Quotient by_splits(n);
+      item.hkv = by_splits.of(unit);
       const int split = unit - item.hkv * n;
-      item.block = of_owner(items) / units - 1 - turn;
+      item.block = Quotient(units).of(of_owner(items)) - 1 - turn;
+      // The first `more` splits have one tile more than the others.
       const int all_tiles = block_tiles<kKind, D>(a, item.seq, item.block);
-      item.begin = static_cast<int>(static_cast<int64_t>(all_tiles) * split / n);
-      item.end = static_cast<int>(static_cast<int64_t>(all_tiles) * (split + 1) / n);
+      const int each = by_splits.of(all_tiles);
+      const int more = all_tiles - each * n;
+      item.begin = each * split + min(split, more);
+      item.end = item.begin + each + (split < more ? 1 : 0);
       item.partial = n > 1;
       item.slot = before_slot + of_owner(from_slot) + at;
       if (item.partial && split == 0) leave(a, item, n);
@@ -225,7 +266,7 @@ struct SequenceLine {
     return Span{block, (n - 1 - block) * pair_length, heavy};
   }
   __device__ __forceinline__ Span span_at(const CachedAttnArgs& a, const Sequence& s, int position) const {
-    const int pair = min(position / pair_length, pairs);
+    const int pair = min(Quotient(pair_length).of(position), pairs);
     const Span heavy = span_of(a, s, n - 1 - pair);
     return pair < pairs && position >= heavy.start + heavy.tiles + kStart ? span_of(a, s, pair) : heavy;
   }
@@ -240,39 +281,47 @@ template <Kind kKind, int D>
 struct Segments {
   int mode, share, chunk, position, end;
   enum { kShares, kLine, kWhole, kDone };
-  __device__ __forceinline__ explicit Segments(const CachedAttnArgs& a)
+  __device__ __forceinline__ Segments(const CachedAttnArgs& a, const Batch& batch)
       : mode(kWhole), share(0), chunk(0), position(0), end(0) {
     // (No block whose partials start here, until there is one.)
     if (threadIdx.x == 0 && static_cast<int>(blockIdx.x) < a.merges) a.merge_blocks[blockIdx.x].splits = 0;
-    const Batch batch(a);
-    const int blocks = a.c.heads_kv * batch.sum([&](const Sequence& s) { return blocks_of<kKind, D>(a, s); });
+    int lane_blocks = 0;
+    int lane_line = 0;
+    float lane_work = 0.f;
+    batch.each([&](const Sequence& s) {
+      const int n = blocks_of<kKind, D>(a, s);
+      lane_blocks += n;
+      lane_work += static_cast<float>(n) * static_cast<float>(tiles_of(s));
+      if (kKind == kWide && a.line) lane_line += SequenceLine<kKind, D>(a, s).length;
+    });
+    const int blocks = a.c.heads_kv * wave_sum(lane_blocks);
     if (blocks == 0 || !batch.sound()) {
       mode = kDone;
       return;
     }
     if (a.num_splits > 0 || a.slots == 0 || blocks > kWholeRounds * a.slots) return;
-    const int total = a.line ? a.c.heads_kv * batch.sum([&](const Sequence& s) {
-      return SequenceLine<kKind, D>(a, s).length;
-    }) : 0;
+    const float work = a.c.heads_kv * wave_sum(lane_work);
+    const int total = a.c.heads_kv * wave_sum(lane_line);
     chunk = max((total + a.slots - 1) / a.slots, a.min_tiles + start_tiles(kKind));
-    share = even_share<kKind, D>(a, batch, blocks, a.slots);
+    share = even_share<kKind, D>(a, batch, blocks, work, a.slots);
     // (A chunk's workgroup starts one more segment than its length counts, and leaves two partials: the line has
     // to gain more than that.)
     if (share > 0 && (!a.line || share <= chunk + 2 * start_tiles(kKind))) {
       mode = kShares;
-    } else if (a.line) {
+    } else if (kKind == kWide && a.line) {
       mode = kLine;
-      position = min(static_cast<int>(blockIdx.x) * chunk, total);  // (chunk <= total / slots + a few)
+      // (There can be more workgroups than slots; blockIdx.x chunk is below total + chunk for those that are not.)
+      position = static_cast<int>(blockIdx.x) < a.slots ? min(static_cast<int>(blockIdx.x) * chunk, total) : total;
       end = min(position + chunk, total);
       position = __builtin_amdgcn_readfirstlane(position);
       end = __builtin_amdgcn_readfirstlane(end);
       chunk = __builtin_amdgcn_readfirstlane(chunk);
     }
   }
-  __device__ __forceinline__ bool next(const CachedAttnArgs& a, Item& item) {
-    if (mode == kDone || (mode == kLine && position >= end)) return false;
-    const Batch batch(a);  // (read again for each segment: kept, it would take registers from the item)
-    if (mode != kLine) {
+  __device__ __forceinline__ bool more() const { return mode != kDone && (mode != kLine || position < end); }
+  __device__ __forceinline__ bool next(const CachedAttnArgs& a, const Batch& batch, Item& item) {
+    if (!more()) return false;
+    if (kKind == kNarrow || mode != kLine) {
       const bool found = find_item<kKind, D>(a, batch, blockIdx.x, share, mode == kWhole, item);
       mode = kDone;
       return found;
@@ -294,7 +343,7 @@ struct Segments {
         item.seq = Sequence{of_owner(s.start), of_owner(s.count), of_owner(s.len)};
         const int origin = of_owner(through) - of_owner(length);  // of the sequence
         const SequenceLine<kKind, D> line(a, item.seq);
-        item.hkv = (position - origin) / line.length;
+        item.hkv = Quotient(line.length).of(position - origin);
         const int start = origin + item.hkv * line.length;  // of the KV head
         const auto span = line.span_at(a, item.seq, position - start);
         item.block = span.block;
@@ -309,7 +358,7 @@ struct Segments {
         const bool any = from == 0 || from < span.tiles;  // (not only what a start costs)
         if (item.partial && from == 0) {
           const int at = position;
-          leave(a, item, -((at + span.tiles - 1) / chunk - static_cast<int>(blockIdx.x) + 1));
+          leave(a, item, -(Quotient(chunk).of(at + span.tiles - 1) - static_cast<int>(blockIdx.x) + 1));
         }
         position = __builtin_amdgcn_readfirstlane(min(end, start + span.start + span.tiles + start_tiles(kKind)));
         if (any) return true;

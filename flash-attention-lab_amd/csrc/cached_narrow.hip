@@ -20,6 +20,7 @@
 //    of the tile, the ones the lane holds; V is read in that order.
 //  * Codes become bf16 or fp16 in registers, with their scales (cache::values4).
 #include "cached.hpp"
+#include "prefill_pp.hpp"
 
 namespace fl {
 namespace cached {
@@ -107,19 +108,6 @@ __device__ __forceinline__ void narrow_item(const CachedAttnArgs& a, const Item&
     const u32x4 x = load16(a.q + q_base + token * a.q_ss + head * a.q_hs + step_dim<kE4M3>(ks, g));
     return in ? x : u32x4{0, 0, 0, 0};
   };
-  u32x4 qf[kQInLds ? 1 : kCols][kSteps];
-  u32x4* q_lds = reinterpret_cast<u32x4*>(smem) + lane;  // [c][ks][64]
-  if constexpr (kQInLds) {
-    for (int i = wave; i < kCols * kSteps; i += kWaves) q_lds[64 * i] = load_q(i / kSteps, i % kSteps);
-    __syncthreads();
-  } else {
-#pragma unroll
-    for (int c = 0; c < kCols; ++c) {
-#pragma unroll
-      for (int ks = 0; ks < kSteps; ++ks) qf[c][ks] = load_q(c, ks);
-    }
-  }
-
   // Lane l works out where the K row (lower half) or V row (upper half) of key l % 32 of a tile lies, and
   // loads its scale.
   const int load_row = lane / P::kPerRow;
@@ -129,7 +117,7 @@ __device__ __forceinline__ void narrow_item(const CachedAttnArgs& a, const Item&
   const char* kp = rows_of(a.c, false, item.b, item.hkv, P::kElem).base + 16 * load_piece;
   const char* vp = rows_of(a.c, true, item.b, item.hkv, P::kElem).base + 16 * load_piece;
   auto first_key = [&](int i) { return (begin + kWaves * i) * kTileKeys; };
-  auto find = [&](int i) { return cache::place(a.c, item.b, min(first_key(i) + (lane & 31), last)); };
+  auto find = [&](int i) { return cache::place(a.c, item.b, max(min(first_key(i) + (lane & 31), last), 0)); };
   u32x4 k[kPieces], v[kPieces];
   uint32_t byte = 0;
   auto load = [&](const cache::Place& p) __attribute__((always_inline)) {
@@ -141,6 +129,30 @@ __device__ __forceinline__ void narrow_item(const CachedAttnArgs& a, const Item&
       v[j] = load16_stream(vp + offsets[32 + load_row + j * kRowStep]);
     }
   };
+
+  // The first tile's loads leave before Q is waited for. (They are made for any item, of no key too.)
+  const cache::Place first = find(0);
+  u32x4 qf[kQInLds ? 1 : kCols][kSteps];
+  u32x4* q_lds = reinterpret_cast<u32x4*>(smem) + lane;  // [c][ks][64]
+  constexpr int kFrags = kCols * kSteps;
+  constexpr int kMine = (kFrags + kWaves - 1) / kWaves;  // that a wave brings into LDS
+  auto my_frag = [&](int i) { return min(kMine * wave + i, kFrags - 1); };
+  if constexpr (kQInLds) {
+    u32x4 mine[kMine];
+#pragma unroll
+    for (int i = 0; i < kMine; ++i) mine[i] = load_q(my_frag(i) / kSteps, my_frag(i) % kSteps);
+    load(first);
+#pragma unroll
+    for (int i = 0; i < kMine; ++i) q_lds[64 * my_frag(i)] = mine[i];
+    prefill::pp::phase_barrier();
+  } else {
+#pragma unroll
+    for (int c = 0; c < kCols; ++c) {
+#pragma unroll
+      for (int ks = 0; ks < kSteps; ++ks) qf[c][ks] = load_q(c, ks);
+    }
+    load(first);
+  }
 
   f32x4 o[kCols][kBlocks];
   float ref[kCols], l[kCols];
@@ -266,11 +278,8 @@ __device__ __forceinline__ void narrow_item(const CachedAttnArgs& a, const Item&
     }
   };
 
-  if (tiles > 0) {
-    load(find(0));
-    at = find(1);
-    for (int i = 0; i < tiles; ++i) step(i);
-  }
+  at = find(1);
+  for (int i = 0; i < tiles; ++i) step(i);
 
   // Merge the four waves in order, 16 rows at a time.
   f32pair* red_ml = reinterpret_cast<f32pair*>(work);                // [kWaves][16]
@@ -351,14 +360,15 @@ __global__ void __launch_bounds__(kThreads)
     cached_narrow_kernel(const CachedAttnArgs a) {
   __shared__ __attribute__((aligned(16))) char smem[kQBytes<D, kCols> + kWorkBytes<D>];
   clear_unowned<D>(a);
-  Segments<kNarrow, D> segments(a);
+  const Batch batch(a);
+  Segments<kNarrow, D> segments(a, batch);
   Item item;
-  if (!segments.next(a, item)) return;
+  if (!segments.next(a, batch, item)) return;
   item = uniform(item);
   if (kMixed && item.seq.count * a.group <= 16) {
-    narrow_item<Tag, D, kE4M3, 1>(a, item, smem);
+    narrow_item<Tag, D, kE4M3, 1>(reload_args(), item, smem);
   } else {
-    narrow_item<Tag, D, kE4M3, kCols>(a, item, smem);
+    narrow_item<Tag, D, kE4M3, kCols>(reload_args(), item, smem);
   }
 }
 

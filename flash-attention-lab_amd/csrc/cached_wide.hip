@@ -461,15 +461,16 @@ __device__ __forceinline__ void pp_item(const CachedAttnArgs& a, const Item& ite
 
   prefill::pp::wait_vmcnt<0>();  // (the loads of tiles past the end have landed before LDS is used again)
   phase_barrier();
+  const CachedAttnArgs& e = reload_args();
   // Rows leave whole: each wave stages its 32 in its own part of the (free) rings, padded by 16 bytes.
   const float lt = sum_halves(l);
-    constexpr int kStageRow = 4 * D + 16;
+  constexpr int kStageRow = 4 * D + 16;
   static_assert(kWaves * 16 * kStageRow <= L::kBytes, "16 rows of each wave fit");
   char* stage = smem + wave * 16 * kStageRow;
   const float inv = inverse(lt);
   if (item.partial) {
     // (In two halves of 16 rows.)
-    float* po = a.partial_o + (a.wide_partials + static_cast<int64_t>(item.slot) * kRows + wave * kWaveRows) * D;
+    float* po = e.partial_o + (e.wide_partials + static_cast<int64_t>(item.slot) * kRows + wave * kWaveRows) * D;
 #pragma unroll
     for (int part = 0; part < 2; ++part) {
       if (((lane >> 4) & 1) == part) {
@@ -492,7 +493,7 @@ __device__ __forceinline__ void pp_item(const CachedAttnArgs& a, const Item& ite
       }
     }
     if (my_row < rows && half == 0)
-      a.partial_ml[a.wide_partials + static_cast<int64_t>(item.slot) * kRows + my_row - q0] = point_and_sum(ref, lt);
+      e.partial_ml[e.wide_partials + static_cast<int64_t>(item.slot) * kRows + my_row - q0] = point_and_sum(ref, lt);
     return;
   }
   constexpr int kOutRow = 2 * D + 16;
@@ -509,20 +510,20 @@ __device__ __forceinline__ void pp_item(const CachedAttnArgs& a, const Item& ite
     }
   }
   constexpr int kLanes = D / 8;  // of a row
-  uint16_t* out = a.o + (a.c.cu_seqlens ? seq.start * a.o_ss : item.b * a.o_bs) + 8 * (lane % kLanes);
+  uint16_t* out = e.o + (e.c.cu_seqlens ? seq.start * e.o_ss : item.b * e.o_bs) + 8 * (lane % kLanes);
 #pragma unroll
   for (int j = 0; j < kWaveRows * kLanes / 64; ++j) {
     const int r = j * (64 / kLanes) + lane / kLanes;
     const u32x4 x = *reinterpret_cast<const u32x4*>(stage + r * kOutRow + 16 * (lane % kLanes));
     if (row0 + r < rows) {
-      const int token = token_of_row(a, row0 + r);
-      const int head = item.hkv * a.group + row0 + r - token * a.group;
-      *reinterpret_cast<u32x4*>(out + token * a.o_ss + head * a.o_hs) = x;
+      const int token = token_of_row(e, row0 + r);
+      const int head = item.hkv * e.group + row0 + r - token * e.group;
+      *reinterpret_cast<u32x4*>(out + token * e.o_ss + head * e.o_hs) = x;
     }
   }
   if (my_row < rows && half == 0) {
-    const int token = token_of_row(a, my_row);
-    a.lse[(static_cast<int64_t>(seq.start) + token) * a.heads + item.hkv * a.group + my_row - token * a.group] =
+    const int token = token_of_row(e, my_row);
+    e.lse[(static_cast<int64_t>(seq.start) + token) * e.heads + item.hkv * e.group + my_row - token * e.group] =
         log_sum(ref, lt);
   }
 }
@@ -531,11 +532,14 @@ template <typename Tag, int D, bool kE4M3>
 __global__ void __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2, 2)))
     cached_wide_kernel(const CachedAttnArgs a) {
   __shared__ __attribute__((aligned(16))) char smem[Lds<D, kE4M3>::kBytes];
-  Segments<kWide, D> segments(a);
+  Batch batch(a);
+  Segments<kWide, D> segments(a, batch);
   Item item;
-  while (segments.next(a, item)) {
-    pp_item<Tag, D, kE4M3>(a, uniform(item), smem);
+  while (segments.next(reload_args(), batch, item)) {
+    pp_item<Tag, D, kE4M3>(reload_args(), uniform(item), smem);
+    if (!segments.more()) break;
     phase_barrier();  // (the next item uses the LDS again)
+    batch.read();     // (kept, it would take registers from the item)
   }
 }
 
