@@ -643,6 +643,9 @@ int check_cached_shape(const fl_cached_attn_params* p) {
     return fail(FL_ERR_INVALID, "query heads must be a multiple of KV heads");
   if (static_cast<int64_t>(p->cache.tokens) * p->heads > INT32_MAX - 256)
     return fail(FL_ERR_INVALID, "tokens * heads too large");
+  // (The kernels count keys to the ends of the tiles that are on their way.)
+  const int64_t capacity = p->cache.block_tables ? static_cast<int64_t>(p->cache.max_blocks) * p->cache.rows : p->cache.rows;
+  if (capacity > INT32_MAX - 1024) return fail(FL_ERR_INVALID, "cache too long for attention_cached (2^31 - 1025 rows)");
   if (p->num_splits < 0 || p->num_splits > fl::kMaxSplits)
     return fail(FL_ERR_INVALID, "num_splits must be in [0, 128]");
   return FL_OK;
@@ -661,7 +664,11 @@ int cached_plan(const fl_cached_attn_params* p, int32_t cu_count, fl::CachedAttn
   a.group_mul = static_cast<uint32_t>((uint64_t{1} << a.group_shift) / static_cast<uint32_t>(a.group) + 1);
   plan = fl::plan_cached_attn(a, p->cache.head_dim, p->cache.dtype == FL_DTYPE_E4M3, cu_count);
   a.wide_partials = plan.wide_partials;
-  if (plan.narrow.workgroups > (int64_t{1} << 24) || plan.wide.workgroups > (int64_t{1} << 24))
+  a.parts[0] = {plan.narrow.slots, plan.narrow.line, plan.narrow.min_tiles, plan.narrow.merges, nullptr};
+  a.parts[1] = {plan.wide.slots, plan.wide.line, plan.wide.min_tiles, plan.wide.merges, nullptr};
+  // (A grid has less than 2^32 threads, 512 and, in the merge, 256 to a workgroup.)
+  constexpr int64_t kMostGroups = (int64_t{1} << 23) - 1;
+  if (plan.narrow.workgroups > kMostGroups || plan.wide.workgroups > kMostGroups || plan.merge_groups > 2 * kMostGroups)
     return fail(FL_ERR_INVALID, "tokens * heads * num_splits exceeds the grid limit");
   return FL_OK;
 }
@@ -940,7 +947,8 @@ int fl_cached_attention(const fl_cached_attn_params* p, int32_t cu_count, fl_str
     if (!aligned(p->workspace, 16)) return fail(FL_ERR_INVALID, "attention workspace must be 16-byte aligned");
     a.partial_o = p->workspace;
     a.partial_ml = reinterpret_cast<fl::f32pair*>(a.partial_o + plan.partial_rows * c.head_dim);
-    a.merge_blocks = reinterpret_cast<fl::MergeBlock*>(a.partial_ml + plan.partial_rows);
+    a.parts[0].merge_blocks = reinterpret_cast<fl::MergeBlock*>(a.partial_ml + plan.partial_rows);
+    a.parts[1].merge_blocks = a.parts[0].merge_blocks + plan.narrow.merges;
   }
   const hipError_t err = fl::launch_cached_attn(a, plan, decode_dtype(p->dtype), c.dtype == FL_DTYPE_E4M3, c.head_dim,
                                                 static_cast<hipStream_t>(stream));

@@ -84,27 +84,30 @@ struct Quotient {
 // The sequences of a batch: lane l holds sequence 64 i + l of chunk i; chunks behind the first are read again
 // in every pass.
 struct Batch {
-  const CachedAttnArgs& a;
+  const CachedAttnArgs* args;
   Sequence first;
-  __device__ __forceinline__ explicit Batch(const CachedAttnArgs& args) : a(args) { read(); }
-  __device__ __forceinline__ void read() { first = at(__lane_id()); }
+  __device__ __forceinline__ explicit Batch(const CachedAttnArgs& a) { read(a); }
+  __device__ __forceinline__ void read(const CachedAttnArgs& a) {
+    args = &a;
+    first = at(__lane_id());
+  }
   __device__ __forceinline__ Sequence at(int b) const {
     Sequence s{0, 0, 0};
-    if (b < a.c.batch) s = cache::sequence(a.c, b);
+    if (b < args->c.batch) s = cache::sequence(args->c, b);
     return s;
   }
   __device__ __forceinline__ Sequence lane_of(int base) const { return base == 0 ? first : at(base + __lane_id()); }
   template <typename F>
   __device__ __forceinline__ void each(F f) const {
     f(first);
-    for (int base = 64; base < a.c.batch; base += 64) f(at(base + __lane_id()));
+    for (int base = 64; base < args->c.batch; base += 64) f(at(base + __lane_id()));
   }
   // Sequences that overlap (cu_seqlens does not ascend) could have more items than the grid and the
   // workspace are made for: no item is run then.
   __device__ __forceinline__ bool sound() const {
-    if (a.c.cu_seqlens == nullptr) return true;
+    if (args->c.cu_seqlens == nullptr) return true;
     bool back = false;
-    for (int b = __lane_id(); b < a.c.batch; b += 64) back |= a.c.cu_seqlens[b + 1] < a.c.cu_seqlens[b];
+    for (int b = __lane_id(); b < args->c.batch; b += 64) back |= args->c.cu_seqlens[b + 1] < args->c.cu_seqlens[b];
     return !wave_any(back);
   }
 };
@@ -146,9 +149,17 @@ __device__ __forceinline__ Item uniform(const Item& i) {
 
 // What the merge needs of a block whose first partial the workgroup leaves (cached_attn.hip): in the workgroup's own
 // place of the list.
+template <Kind kKind>
 __device__ __forceinline__ void leave(const CachedAttnArgs& a, const Item& item, int splits) {
-  if (threadIdx.x == 0 && static_cast<int>(blockIdx.x) < a.merges)
-    a.merge_blocks[blockIdx.x] = MergeBlock{splits, item.slot, item.b, item.hkv, item.block, item.seq.start, item.seq.count, 0};
+  if (threadIdx.x == 0 && static_cast<int>(blockIdx.x) < a.parts[kKind].merges)
+    a.parts[kKind].merge_blocks[blockIdx.x] = MergeBlock{splits, item.slot, item.b, item.hkv, item.block, item.seq.start, item.seq.count, 0};
+}
+
+// No block whose partials start with this workgroup, until there is one. Every kernel does this first of all.
+template <Kind kKind>
+__device__ __forceinline__ void clear_list(const CachedAttnArgs& a) {
+  if (threadIdx.x == 0 && static_cast<int>(blockIdx.x) < a.parts[kKind].merges)
+    a.parts[kKind].merge_blocks[blockIdx.x].splits = 0;
 }
 
 // Items of equal shares: sequence b has blocks_b splits_b H_kv of them, with splits_b = ceil(tiles_b / share).
@@ -163,7 +174,7 @@ __device__ __forceinline__ int even_share(const CachedAttnArgs& a, const Batch& 
     return a.c.heads_kv * wave_sum(total);
   };
   // sum of ceil(x / t) is at most work / t + blocks.
-  int low = max(a.min_tiles, static_cast<int>(work / slots));
+  int low = max(a.parts[kKind].min_tiles, static_cast<int>(work / slots));
   int high = blocks < slots ? max(low, static_cast<int>(work / (slots - blocks) * 1.001f) + 1) : 1 << 28;
   while (low < high) {
     const int mid = low + (high - low) / 2;
@@ -230,7 +241,7 @@ __device__ __forceinline__ bool find_item(const CachedAttnArgs& a, const Batch& 
       item.end = item.begin + each + (split < more ? 1 : 0);
       item.partial = n > 1;
       item.slot = before_slot + of_owner(from_slot) + at;
-      if (item.partial && split == 0) leave(a, item, n);
+      if (item.partial && split == 0) leave<kKind>(a, item, n);
       return true;
     }
     before += __builtin_amdgcn_readlane(all, 63);
@@ -279,12 +290,10 @@ struct SequenceLine {
 //  * whole blocks as they come, where there are many rounds of them (or no workspace).
 template <Kind kKind, int D>
 struct Segments {
-  int mode, share, chunk, position, end;
   enum { kShares, kLine, kWhole, kDone };
+  int mode, share, chunk, position, end;
   __device__ __forceinline__ Segments(const CachedAttnArgs& a, const Batch& batch)
       : mode(kWhole), share(0), chunk(0), position(0), end(0) {
-    // (No block whose partials start here, until there is one.)
-    if (threadIdx.x == 0 && static_cast<int>(blockIdx.x) < a.merges) a.merge_blocks[blockIdx.x].splits = 0;
     int lane_blocks = 0;
     int lane_line = 0;
     float lane_work = 0.f;
@@ -292,26 +301,26 @@ struct Segments {
       const int n = blocks_of<kKind, D>(a, s);
       lane_blocks += n;
       lane_work += static_cast<float>(n) * static_cast<float>(tiles_of(s));
-      if (kKind == kWide && a.line) lane_line += SequenceLine<kKind, D>(a, s).length;
+      if (kKind == kWide && a.parts[kKind].line) lane_line += SequenceLine<kKind, D>(a, s).length;
     });
     const int blocks = a.c.heads_kv * wave_sum(lane_blocks);
     if (blocks == 0 || !batch.sound()) {
       mode = kDone;
       return;
     }
-    if (a.num_splits > 0 || a.slots == 0 || blocks > kWholeRounds * a.slots) return;
+    if (a.num_splits > 0 || a.parts[kKind].slots == 0 || blocks > kWholeRounds * a.parts[kKind].slots) return;
     const float work = a.c.heads_kv * wave_sum(lane_work);
     const int total = a.c.heads_kv * wave_sum(lane_line);
-    chunk = max((total + a.slots - 1) / a.slots, a.min_tiles + start_tiles(kKind));
-    share = even_share<kKind, D>(a, batch, blocks, work, a.slots);
+    chunk = max((total + a.parts[kKind].slots - 1) / a.parts[kKind].slots, a.parts[kKind].min_tiles + start_tiles(kKind));
+    share = even_share<kKind, D>(a, batch, blocks, work, a.parts[kKind].slots);
     // (A chunk's workgroup starts one more segment than its length counts, and leaves two partials: the line has
     // to gain more than that.)
-    if (share > 0 && (!a.line || share <= chunk + 2 * start_tiles(kKind))) {
+    if (share > 0 && (!a.parts[kKind].line || share <= chunk + 2 * start_tiles(kKind))) {
       mode = kShares;
-    } else if (kKind == kWide && a.line) {
+    } else if (kKind == kWide && a.parts[kKind].line) {
       mode = kLine;
       // (There can be more workgroups than slots; blockIdx.x chunk is below total + chunk for those that are not.)
-      position = static_cast<int>(blockIdx.x) < a.slots ? min(static_cast<int>(blockIdx.x) * chunk, total) : total;
+      position = static_cast<int>(blockIdx.x) < a.parts[kKind].slots ? min(static_cast<int>(blockIdx.x) * chunk, total) : total;
       end = min(position + chunk, total);
       position = __builtin_amdgcn_readfirstlane(position);
       end = __builtin_amdgcn_readfirstlane(end);
@@ -358,7 +367,7 @@ struct Segments {
         const bool any = from == 0 || from < span.tiles;  // (not only what a start costs)
         if (item.partial && from == 0) {
           const int at = position;
-          leave(a, item, -(Quotient(chunk).of(at + span.tiles - 1) - static_cast<int>(blockIdx.x) + 1));
+          leave<kKind>(a, item, -(Quotient(chunk).of(at + span.tiles - 1) - static_cast<int>(blockIdx.x) + 1));
         }
         position = __builtin_amdgcn_readfirstlane(min(end, start + span.start + span.tiles + start_tiles(kKind)));
         if (any) return true;
@@ -409,6 +418,51 @@ __device__ __forceinline__ f32pair point_and_sum(float ref, float l) {
 }
 __device__ __forceinline__ float inverse(float l) { return l == 0.f ? 0.f : 1.f / l; }
 __device__ __forceinline__ float log_sum(float ref, float l) { return l == 0.f ? -INFINITY : ref * kLn2 + logf(l); }
+
+// Four consecutive dims of row `key` of a sequence's K (or V), from the one that `at` bytes lead to.
+template <typename Tag, bool kE4M3>
+__device__ __forceinline__ f32x4 four_of(const CacheArgs& c, const RowSpace& rows, const RowSpace& scales,
+                                         const cache::Place& p, int dim) {
+  u32x2 x;
+  if constexpr (kE4M3) {
+    const uint32_t codes = *reinterpret_cast<const uint32_t*>(rows.base + rows.offset(c, p) + dim);
+    x = cache::values4<Tag>(codes, cache::scale_of(static_cast<uint8_t>(scales.base[scales.offset(c, p)])));
+  } else {
+    x = *reinterpret_cast<const u32x2*>(rows.base + rows.offset(c, p) + 2 * dim);
+  }
+  using E = Elem<Tag>;
+  return f32x4{E::to_float(x.x & 0xffff), E::to_float(x.x >> 16), E::to_float(x.y & 0xffff), E::to_float(x.y >> 16)};
+}
+
+// A value that is not finite reaches the rows that do not see its key too, where they share a tile with rows that
+// do: 0 times it is NaN. Rows of a causal call whose sum is not finite are therefore summed again, over their own
+// keys alone: the sum over the item's keys of 2^(s - ref) v, by D / 4 lanes with four dims each. (Slow, a key at a
+// time; reached only with such values in the cache.)
+template <typename Tag, int D, bool kE4M3>
+__device__ __forceinline__ f32x4 sum_again(const CachedAttnArgs& a, const Item& item, int row, float ref, int lane) {
+  using E = Elem<Tag>;
+  constexpr int kLanes = D / 4;
+  constexpr int kElem = kE4M3 ? 1 : 2;
+  const int dim = 4 * (lane % kLanes);
+  const int token = token_of_row(a, row);
+  const int head = item.hkv * a.group + row - token * a.group;
+  const int64_t q_row = a.c.cu_seqlens ? (item.seq.start + token) * a.q_ss : item.b * a.q_bs + token * a.q_ss;
+  const u32x2 q = *reinterpret_cast<const u32x2*>(a.q + q_row + head * a.q_hs + dim);
+  const RowSpace k = rows_of(a.c, false, item.b, item.hkv, kElem), v = rows_of(a.c, true, item.b, item.hkv, kElem);
+  const RowSpace ks = scales_of(a.c, false, item.b, item.hkv), vs = scales_of(a.c, true, item.b, item.hkv);
+  const int end = min(min(item.end * kKeys, item.seq.len), item.seq.len - item.seq.count + token + 1);
+  f32x4 o = {};
+  for (int key = item.begin * kKeys; key < end; ++key) {
+    const cache::Place p = cache::place(a.c, item.b, key);
+    const f32x4 x = four_of<Tag, kE4M3>(a.c, k, ks, p, dim);
+    float s = E::to_float(q.x & 0xffff) * x[0] + E::to_float(q.x >> 16) * x[1] + E::to_float(q.y & 0xffff) * x[2] +
+              E::to_float(q.y >> 16) * x[3];
+#pragma unroll
+    for (int m = kLanes / 2; m >= 1; m /= 2) s += __shfl_xor(s, m);
+    o += four_of<Tag, kE4M3>(a.c, v, vs, p, dim) * exp2_fast(fmaf(s, a.scale_log2, -ref));
+  }
+  return o;
+}
 
 }  // namespace
 }  // namespace cached

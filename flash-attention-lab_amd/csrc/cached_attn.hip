@@ -29,7 +29,7 @@ template <int D>
 constexpr int kMergeRows = kMergeThreads / (D / 4);
 template <typename Tag, int D>
 __global__ void __launch_bounds__(kMergeThreads)
-    cached_merge_kernel(const CachedAttnArgs a, const MergeBlock* wide_blocks, int narrow_groups, int narrow_chunks) {
+    cached_merge_kernel(const CachedAttnArgs a, int narrow_groups, int narrow_chunks) {
   using E = Elem<Tag>;
   constexpr int kLanes = D / 4;
   constexpr int kGroups = kMergeRows<D>;
@@ -40,7 +40,7 @@ __global__ void __launch_bounds__(kMergeThreads)
   const int chunks = wide ? block_rows(kWide) / kGroups : narrow_chunks;
   const int at = id / chunks;
   const int chunk = id - at * chunks;
-  const MergeBlock mb = (wide ? wide_blocks : a.merge_blocks)[at];
+  const MergeBlock mb = a.parts[wide ? kWide : kNarrow].merge_blocks[at];
   if (mb.splits == 0) return;
   const int per_block = wide ? block_rows(kWide) : kNarrowRows;
   const int rows = min(per_block, mb.count * a.group - mb.block * per_block);
@@ -100,14 +100,21 @@ __global__ void __launch_bounds__(kMergeThreads)
   if (d == 0) a.lse[(static_cast<int64_t>(mb.start) + token) * a.heads + head] = log_sum(m, l);
 }
 
+// Workgroups of a narrow block, and of all.
+int64_t narrow_chunks(const CachedPlan& plan, int head_dim) {
+  const int rows = kMergeThreads / (head_dim / 4);
+  return ((plan.most_rows < kNarrowRows ? plan.most_rows : kNarrowRows) + rows - 1) / rows;
+}
+int64_t merge_groups(const CachedPlan& plan, int head_dim) {
+  return plan.narrow.merges * narrow_chunks(plan, head_dim) +
+         plan.wide.merges * int64_t{block_rows(kWide) / (kMergeThreads / (head_dim / 4))};
+}
+
 template <typename Tag, int D>
 hipError_t launch_merge(const CachedAttnArgs& args, const CachedPlan& plan, hipStream_t stream) {
-  const int most = plan.most_rows < kNarrowRows ? plan.most_rows : kNarrowRows;
-  const int narrow_chunks = (most + kMergeRows<D> - 1) / kMergeRows<D>;
-  const int narrow_groups = plan.narrow.merges * narrow_chunks;
-  const int wide_groups = plan.wide.merges * (block_rows(kWide) / kMergeRows<D>);
-  hipLaunchKernelGGL((cached_merge_kernel<Tag, D>), dim3(narrow_groups + wide_groups), dim3(kMergeThreads), 0, stream,
-                     args, args.merge_blocks + plan.narrow.merges, narrow_groups, narrow_chunks);
+  const int chunks = static_cast<int>(narrow_chunks(plan, D));
+  hipLaunchKernelGGL((cached_merge_kernel<Tag, D>), dim3(static_cast<uint32_t>(plan.merge_groups)), dim3(kMergeThreads), 0,
+                     stream, args, plan.narrow.merges * chunks, chunks);
   return hipGetLastError();
 }
 
@@ -134,15 +141,6 @@ CachedPlan::Part plan_part(const CachedAttnArgs& args, Kind kind, int64_t least,
   return part;
 }
 
-CachedAttnArgs with_part(CachedAttnArgs args, const CachedPlan::Part& part, int64_t blocks_before) {
-  args.merge_blocks += blocks_before;
-  args.merges = part.merges;
-  args.slots = part.slots;
-  args.line = part.line;
-  args.min_tiles = part.min_tiles;
-  return args;
-}
-
 }  // namespace
 }  // namespace cached
 
@@ -160,11 +158,14 @@ CachedPlan plan_cached_attn(const CachedAttnArgs& args, int head_dim, bool e4m3,
   // its launch 6.4 us and more with what else is read (one split / several, e4m3: B = 1, 32/8 heads, 640 keys 10.4
   // us / 6.9 + 4.7, 1,024 13.6 / 7.0 + 4.6; B = 16, 1,024 keys 17.5 / 13.3 + 4.2, 1,536 22.5 / 15.3 + 4.1).
   const double megabytes = 2e-6 * c.batch * c.heads_kv * c.capacity * head_dim * (e4m3 ? 1 : 2);
-  const bool whole = plan.most_rows <= kNarrowRows && 7.2e-3 * c.capacity < 6.4 + 0.08 * megabytes;
+  plan.whole = plan.most_rows <= kNarrowRows && 7.2e-3 * c.capacity < 6.4 + 0.08 * megabytes;
   if (ragged || per_seq <= kNarrowRows) {
     const int64_t least = ragged ? 0 : c.batch * int64_t{c.heads_kv};
+    // (In the kernel of the wide ones a workgroup has twice the waves, and a CU to itself.)
+    const bool with_wide = plan.most_rows > kNarrowRows;
     plan.narrow = plan_part(args, kNarrow, least, c.batch * int64_t{c.heads_kv},
-                            cus * cached_narrow_resident(head_dim, e4m3, plan.most_rows), 2, whole);
+                            cus * (with_wide ? 1 : cached_narrow_resident(head_dim, e4m3, plan.most_rows)),
+                            with_wide ? 4 : 2, plan.whole);
   }
   if (plan.most_rows > kNarrowRows) {
     const int64_t wide_rows = block_rows(kWide);
@@ -178,17 +179,15 @@ CachedPlan plan_cached_attn(const CachedAttnArgs& args, int head_dim, bool e4m3,
   plan.partial_rows = plan.wide_partials + plan.wide.partials * block_rows(kWide);
   plan.floats = plan.partial_rows * (head_dim + 2) +
                 (plan.narrow.merges + static_cast<int64_t>(plan.wide.merges)) * (sizeof(MergeBlock) / sizeof(float));
+  plan.merge_groups = merge_groups(plan, head_dim);
   return plan;
 }
 
 hipError_t launch_cached_attn(const CachedAttnArgs& args, const CachedPlan& plan, DType dtype, bool e4m3,
                               int head_dim, hipStream_t stream) {
   using namespace cached;
-  hipError_t err = hipSuccess;
-  if (plan.wide.workgroups > 0)
-    err = launch_cached_wide(with_part(args, plan.wide, plan.narrow.merges), plan.wide.workgroups, dtype, e4m3, head_dim, stream);
-  if (err == hipSuccess && plan.narrow.workgroups > 0)
-    err = launch_cached_narrow(with_part(args, plan.narrow, 0), plan, dtype, e4m3, head_dim, stream);
+  const hipError_t err = plan.wide.workgroups > 0 ? launch_cached_wide(args, plan, dtype, e4m3, head_dim, stream)
+                                                  : launch_cached_narrow(args, plan, dtype, e4m3, head_dim, stream);
   if (err != hipSuccess || plan.partial_rows == 0) return err;
   if (head_dim == 64) {
     return dtype == DType::bf16 ? launch_merge<bf16_tag, 64>(args, plan, stream)

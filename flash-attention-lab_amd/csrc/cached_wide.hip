@@ -12,8 +12,7 @@
 //    per workgroup.
 //  * A workgroup has one item, a share of a block's tiles (cached.hpp), and the rows of all query heads of
 //    a KV head.
-#include "cached.hpp"
-#include "prefill_pp.hpp"
+#include "cached_narrow.hpp"
 
 namespace fl {
 namespace cached {
@@ -462,6 +461,36 @@ __device__ __forceinline__ void pp_item(const CachedAttnArgs& a, const Item& ite
   prefill::pp::wait_vmcnt<0>();  // (the loads of tiles past the end have landed before LDS is used again)
   phase_barrier();
   const CachedAttnArgs& e = reload_args();
+  // Rows to sum again (sum_again): both halves of a row's lanes say which.
+  uint32_t again = 0;
+  if (e.causal && seq.count > 1) {
+    float sum = 0.f;
+#pragma unroll
+    for (int nb = 0; nb < D / 32; ++nb) {
+#pragma unroll
+      for (int j = 0; j < 16; ++j) sum = fmaf(o[nb][j], 0.f, sum);
+    }
+    const uint64_t bad = __builtin_amdgcn_ballot_w64(sum != 0.f && my_row < rows);
+    again = static_cast<uint32_t>(bad) | static_cast<uint32_t>(bad >> 32);
+  }
+  // f(row of the wave, its reference point, its sum, its four dims, which of them) for those rows, when the wave's stores have
+  // been made.
+  auto each_again = [&](float lt, auto&& f) {
+    if (again == 0) return;
+    prefill::pp::wait_vmcnt<0>();
+    int lane = threadIdx.x & 63;
+    asm volatile("" : "+v"(lane));  // (as tid)
+    const int lane_dim = 4 * (lane % (D / 4));
+    while (again != 0) {
+      const int r = __builtin_ctz(again);
+      again &= again - 1;
+      const float row_ref = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(ref), r));
+      const float row_sum = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(lt), r));
+      if (row_sum != row_sum) continue;  // (NaN whatever V is)
+      const f32x4 x = sum_again<Tag, D, kE4M3>(reload_args(), item, row0 + r, row_ref, lane);
+      if (lane < D / 4) f(r, row_sum, x, lane_dim);
+    }
+  };
   // Rows leave whole: each wave stages its 32 in its own part of the (free) rings, padded by 16 bytes.
   const float lt = sum_halves(l);
   constexpr int kStageRow = 4 * D + 16;
@@ -494,6 +523,7 @@ __device__ __forceinline__ void pp_item(const CachedAttnArgs& a, const Item& ite
     }
     if (my_row < rows && half == 0)
       e.partial_ml[e.wide_partials + static_cast<int64_t>(item.slot) * kRows + my_row - q0] = point_and_sum(ref, lt);
+    each_again(lt, [&](int r, float, const f32x4& x, int dim) { *reinterpret_cast<f32x4*>(po + r * D + dim) = x; });
     return;
   }
   constexpr int kOutRow = 2 * D + 16;
@@ -526,30 +556,100 @@ __device__ __forceinline__ void pp_item(const CachedAttnArgs& a, const Item& ite
     e.lse[(static_cast<int64_t>(seq.start) + token) * e.heads + item.hkv * e.group + my_row - token * e.group] =
         log_sum(ref, lt);
   }
+  each_again(lt, [&](int r, float row_sum, const f32x4& x, int dim) {
+    const float row_inv = inverse(row_sum);
+    const int token = token_of_row(e, row0 + r);
+    const int head = item.hkv * e.group + row0 + r - token * e.group;
+    *reinterpret_cast<u32x2*>(e.o + (e.c.cu_seqlens ? seq.start * e.o_ss : item.b * e.o_bs) + token * e.o_ss +
+                              head * e.o_hs + dim) =
+        u32x2{E::pack2(x[0] * row_inv, x[1] * row_inv), E::pack2(x[2] * row_inv, x[3] * row_inv)};
+  });
 }
 
+// The narrow sequences of a ragged batch run in the same launch: each workgroup takes its share of them too, with
+// eight waves, every other workgroup first of all. So one half of the chip reads the cache while the other is on
+// the matrix cores. (Two launches took 4.4 us more, where one had nothing to do.)
+constexpr int kNarrowCols = (kNarrowRows + 15) / 16;
+
 template <typename Tag, int D, bool kE4M3>
-__global__ void __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2, 2)))
-    cached_wide_kernel(const CachedAttnArgs a) {
-  __shared__ __attribute__((aligned(16))) char smem[Lds<D, kE4M3>::kBytes];
-  Batch batch(a);
+__device__ __forceinline__ void run_wide(Batch& batch, char* smem) {
+  const CachedAttnArgs& a = reload_args();
+  batch.args = &a;
   Segments<kWide, D> segments(a, batch);
   Item item;
   while (segments.next(reload_args(), batch, item)) {
     pp_item<Tag, D, kE4M3>(reload_args(), uniform(item), smem);
     if (!segments.more()) break;
     phase_barrier();  // (the next item uses the LDS again)
-    batch.read();     // (kept, it would take registers from the item)
+    batch.read(reload_args());  // (kept, it would take registers from the item)
+  }
+}
+
+template <typename Tag, int D, bool kE4M3>
+__device__ __forceinline__ void run_narrow(Batch& batch, char* smem) {
+  const CachedAttnArgs& a = reload_args();
+  batch.args = &a;
+  Segments<kNarrow, D> segments(a, batch);
+  Item item;
+  if (!segments.next(a, batch, item)) return;
+  item = uniform(item);
+  if (item.seq.count * a.group <= 16) {
+    narrow_item<Tag, D, kE4M3, 1, kWaves>(reload_args(), item, smem);
+  } else {
+    narrow_item<Tag, D, kE4M3, kNarrowCols, kWaves>(reload_args(), item, smem);
+  }
+}
+
+template <typename Tag, int D, bool kE4M3, bool kRagged>
+__global__ void __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2, 2)))
+    cached_wide_kernel(const CachedAttnArgs a) {
+  constexpr int kBytes = Lds<D, kE4M3>::kBytes, kNarrowBytes = NarrowLds<D, kNarrowCols, kWaves>::kBytes;
+  __shared__ __attribute__((aligned(16))) char smem[kRagged && kNarrowBytes > kBytes ? kNarrowBytes : kBytes];
+  Batch batch(a);
+  clear_list<kWide>(a);
+  if constexpr (!kRagged) {
+    run_wide<Tag, D, kE4M3>(batch, smem);
+  } else {
+    clear_list<kNarrow>(a);
+    clear_unowned<D>(a);
+    bool lane_narrow = false;
+    bool lane_wide = false;
+    batch.each([&](const Sequence& s) {
+      lane_narrow |= blocks_of<kNarrow, D>(a, s) > 0;
+      lane_wide |= blocks_of<kWide, D>(a, s) > 0;
+    });
+    const bool any[2] = {wave_any(lane_narrow), wave_any(lane_wide)};
+    const int narrow_at = any[kWide] ? (blockIdx.x >> 3) & 1 : 0;  // (neighbours run on different XCDs)
+    for (int i = 0; i < 2; ++i) {
+      if (i == narrow_at) {
+        if (any[kNarrow]) run_narrow<Tag, D, kE4M3>(batch, smem);
+      } else {
+        if (any[kWide]) run_wide<Tag, D, kE4M3>(batch, smem);
+      }
+      if (i == 1 || !any[kNarrow] || !any[kWide]) continue;
+      phase_barrier();  // (the other part uses the LDS again)
+      batch.read(reload_args());  // (kept, it would take registers from the items)
+    }
+  }
+}
+
+template <typename Tag, int D, bool kE4M3>
+void launch_ragged_or_not(const CachedAttnArgs& args, const CachedPlan& plan, hipStream_t stream) {
+  if (args.c.cu_seqlens != nullptr) {
+    const int64_t most = plan.wide.workgroups > plan.narrow.workgroups ? plan.wide.workgroups : plan.narrow.workgroups;
+    hipLaunchKernelGGL((cached_wide_kernel<Tag, D, kE4M3, true>), dim3(static_cast<uint32_t>(most)), dim3(kThreads), 0, stream, args);
+  } else {
+    hipLaunchKernelGGL((cached_wide_kernel<Tag, D, kE4M3, false>), dim3(static_cast<uint32_t>(plan.wide.workgroups)), dim3(kThreads), 0,
+                       stream, args);
   }
 }
 
 template <typename Tag, int D>
-hipError_t launch_typed(const CachedAttnArgs& args, int64_t workgroups, bool e4m3, hipStream_t stream) {
-  const dim3 grid(static_cast<uint32_t>(workgroups));
+hipError_t launch_typed(const CachedAttnArgs& args, const CachedPlan& plan, bool e4m3, hipStream_t stream) {
   if (e4m3) {
-    hipLaunchKernelGGL((cached_wide_kernel<Tag, D, true>), grid, dim3(kThreads), 0, stream, args);
+    launch_ragged_or_not<Tag, D, true>(args, plan, stream);
   } else {
-    hipLaunchKernelGGL((cached_wide_kernel<Tag, D, false>), grid, dim3(kThreads), 0, stream, args);
+    launch_ragged_or_not<Tag, D, false>(args, plan, stream);
   }
   return hipGetLastError();
 }
@@ -557,15 +657,15 @@ hipError_t launch_typed(const CachedAttnArgs& args, int64_t workgroups, bool e4m
 }  // namespace
 }  // namespace cached
 
-hipError_t launch_cached_wide(const CachedAttnArgs& args, int64_t workgroups, DType dtype, bool e4m3, int head_dim,
+hipError_t launch_cached_wide(const CachedAttnArgs& args, const CachedPlan& plan, DType dtype, bool e4m3, int head_dim,
                               hipStream_t stream) {
   using namespace cached;
   if (dtype == DType::bf16) {
-    return head_dim == 64 ? launch_typed<bf16_tag, 64>(args, workgroups, e4m3, stream)
-                          : launch_typed<bf16_tag, 128>(args, workgroups, e4m3, stream);
+    return head_dim == 64 ? launch_typed<bf16_tag, 64>(args, plan, e4m3, stream)
+                          : launch_typed<bf16_tag, 128>(args, plan, e4m3, stream);
   }
-  return head_dim == 64 ? launch_typed<f16_tag, 64>(args, workgroups, e4m3, stream)
-                        : launch_typed<f16_tag, 128>(args, workgroups, e4m3, stream);
+  return head_dim == 64 ? launch_typed<f16_tag, 64>(args, plan, e4m3, stream)
+                        : launch_typed<f16_tag, 128>(args, plan, e4m3, stream);
 }
 
 }  // namespace fl

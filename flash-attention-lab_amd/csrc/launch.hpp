@@ -142,17 +142,19 @@ struct CachedAttnArgs {
   uint32_t group_mul;
   int group_shift;
   int num_splits;  // forced, or 0
-  // Of the kind of sequences that a kernel runs (cached.hpp):
-  int slots;       // workgroups that run at once, where keys may be split; 0: no splits
-  int line;        // whether they may share a line (cached.hpp)
-  int min_tiles;   // fewest key tiles of a split
+  // Of the narrow and the wide sequences (cached.hpp):
+  struct Part {
+    int slots;      // workgroups that run at once, where keys may be split; 0: no splits
+    int line;       // whether they may share a line
+    int min_tiles;  // fewest key tiles of a split
+    int merges;     // entries of the list
+    MergeBlock* merge_blocks;
+  } parts[2];
   // Partials: [slot][row of the block], the narrow sequences' slots first, the wide ones' from row
   // wide_partials on.
   int64_t wide_partials;
   float* partial_o;       // [D] unnormalized
   f32pair* partial_ml;    // (reference point in log2 units or -inf, sum)
-  MergeBlock* merge_blocks;  // of this kind
-  int merges;
 };
 
 // How the decode kernels find cache rows: contiguous cache, paged cache with the split's block
@@ -236,16 +238,19 @@ struct CachedPlan {
   };
   Part narrow, wide;  // workgroups 0: there are none of the kind
   int most_rows;      // of a sequence
+  bool whole;         // narrow blocks are not split
   int64_t wide_partials, partial_rows, floats;
+  int64_t merge_groups;  // workgroups of the merge
 };
 CachedPlan plan_cached_attn(const CachedAttnArgs& args, int head_dim, bool e4m3, int cu_count);
 hipError_t launch_cached_attn(const CachedAttnArgs& args, const CachedPlan& plan, DType dtype, bool e4m3,
                               int head_dim, hipStream_t stream);
-// Its kernels (cached_narrow.hip, cached_wide.hip), and how many workgroups of the first a CU holds.
+// Its kernels (cached_narrow.hip; cached_wide.hip, which runs a ragged batch's narrow sequences too), and how many
+// workgroups of the first a CU holds.
 int cached_narrow_resident(int head_dim, bool e4m3, int most_rows);
 hipError_t launch_cached_narrow(const CachedAttnArgs& args, const CachedPlan& plan, DType dtype, bool e4m3,
                                 int head_dim, hipStream_t stream);
-hipError_t launch_cached_wide(const CachedAttnArgs& args, int64_t workgroups, DType dtype, bool e4m3, int head_dim,
+hipError_t launch_cached_wide(const CachedAttnArgs& args, const CachedPlan& plan, DType dtype, bool e4m3, int head_dim,
                               hipStream_t stream);
 
 hipError_t launch_axpy(const float* x, const float* y, float alpha, float* out, int64_t n,

@@ -262,3 +262,21 @@ def test_struct_layouts():
     assert ctypes.sizeof(_hip.KvCache) == 200
     assert ctypes.sizeof(_hip.TokenRows) == 72
     assert ctypes.sizeof(_hip.CachedAttnParams) == 312
+
+
+def test_c_attention_refuses_sizes_beyond_its_counters():
+    call = lambda p: _hip.LIB.fl_cached_attention(ctypes.byref(p), 256, None)
+    far = 1 << 32
+    refused(call(c_attn(c_cache(k_seq_stride=far))), "stride too large")
+    pool = dict(block_tables=256, max_blocks=4)
+    refused(call(c_attn(c_cache(v_batch_stride=far, **pool))), "stride too large")
+    codes = dict(dtype=3, k_scales=256, v_scales=256)
+    refused(call(c_attn(c_cache(ks_seq_stride=far, **codes))), "scales stride too large")
+    refused(call(c_attn(c_cache(block_tables=256, max_blocks=(1 << 31) // 40))), "cache too long")
+    refused(call(c_attn(c_cache(rows=(1 << 31) - 1))), "cache too long")
+    # A grid has less than 2^32 threads, that of the merge too.
+    refused(call(c_attn(c_cache(tokens=1 << 26), heads=16, num_splits=128)), "grid limit")
+    refused(call(c_attn(c_cache(batch=1 << 17, outer=1 << 17, tokens=1 << 17), heads=2, num_splits=128)), "grid limit")
+    size = ctypes.c_size_t()
+    refused(_hip.LIB.fl_cached_attention_plan(ctypes.byref(c_attn(c_cache(tokens=1 << 26), heads=16, num_splits=128)), 256,
+                                              ctypes.byref(size)), "grid limit")
