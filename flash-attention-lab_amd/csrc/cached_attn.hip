@@ -154,11 +154,15 @@ CachedPlan plan_cached_attn(const CachedAttnArgs& args, int head_dim, bool e4m3,
   CachedPlan plan{};
   // Rows of the largest sequence there can be, which kinds there can be, and their blocks.
   plan.most_rows = static_cast<int>(ragged ? rows : per_seq);
-  // Short caches of one kind keep their blocks whole: a workgroup takes about 7.2 us for 1,000 keys, the merge and
-  // its launch 6.4 us and more with what else is read (one split / several, e4m3: B = 1, 32/8 heads, 640 keys 10.4
-  // us / 6.9 + 4.7, 1,024 13.6 / 7.0 + 4.6; B = 16, 1,024 keys 17.5 / 13.3 + 4.2, 1,536 22.5 / 15.3 + 4.1).
+  // Short caches keep their blocks whole, one workgroup each (of eight waves, with up to 16 rows): its time goes up
+  // by 5.3 us for 1,000 keys (9.5 with more rows, on four waves), a merge and its launch cost 5.5 us (7). In a large
+  // batch splits gain less than that from longer caches too; but lengths can differ, which whole blocks do not even
+  // out, so only part of it counts. us, whole / split + merge, 32/8 heads, head_dim 128, e4m3: B = 1, 640 keys 9.1 /
+  // 6.5 + 4.1, 1,024 11.5 / 6.7 + 4.4, 1,536 14.3 / 6.5 + 4.7; B = 16, 1,024 14.6 / 12.6 + 4.4, 2,048 22.5 / 18.4 + 4.5;
+  // bf16, B = 16, 2,048 32.0 / 29.6 + 4.1; 8 tokens each, e4m3: B = 1, 640 13.6 / 8.9 + 4.4, B = 16, 1,024 19.1 / 19.2 + 6.4.
   const double megabytes = 2e-6 * c.batch * c.heads_kv * c.capacity * head_dim * (e4m3 ? 1 : 2);
-  plan.whole = plan.most_rows <= kNarrowRows && 7.2e-3 * c.capacity < 6.4 + 0.08 * megabytes;
+  plan.whole = plan.most_rows <= 16 ? 5.3e-3 * c.capacity < 5.5 + 0.06 * megabytes
+                                    : plan.most_rows <= kNarrowRows && 9.5e-3 * c.capacity < 7.0 + 0.1 * megabytes;
   if (ragged || per_seq <= kNarrowRows) {
     const int64_t least = ragged ? 0 : c.batch * int64_t{c.heads_kv};
     // (In the kernel of the wide ones a workgroup has twice the waves, and a CU to itself.)
