@@ -1,7 +1,6 @@
-// Pieces shared by the kernels of attention over a cache (cached_attn.hip: plan and merge; cached_narrow.hip:
-// sequences with few rows; cached_wide.hip: the
-// others): the rows of a sequence, the items that the
-// workgroups of a kernel share out, and the offsets of cache rows.
+// Pieces shared by the kernels of attention over a cache (cached_attn.hip: plan and merge; cached_narrow.hpp:
+// sequences with few rows; cached_wide.hip: the others, and ragged batches of both): the rows of a sequence, the
+// items of work that workgroups share out, and the offsets of cache rows.
 #pragma once
 
 #include <type_traits>
@@ -17,8 +16,9 @@ namespace cached {
 enum Kind { kNarrow, kWide };
 constexpr int kNarrowRows = 48;  // most rows of a narrow sequence
 constexpr int kKeys = 64;        // keys of a tile: splits are whole tiles
-// Tiles that starting and ending an item costs as much as.
-__host__ __device__ __forceinline__ constexpr int start_tiles(Kind kind) { return kind == kNarrow ? 4 : 6; }
+// Tiles that starting and ending an item of a wide block costs as much as (about 7 us before the first tile is done
+// and 2 us behind the last, at 2 us a tile of 16-bit keys at head_dim 128).
+constexpr int kStartTiles = 6;
 // From so many rounds of blocks on they run whole, as they come, the longest first.
 constexpr int kWholeRounds = 6;
 // Rows of a block.
@@ -258,7 +258,7 @@ __device__ __forceinline__ bool find_item(const CachedAttnArgs& a, const Batch& 
 template <Kind kKind, int D>
 struct SequenceLine {
   int n, pairs, pair_tiles, pair_length, length;  // blocks, pairs, tiles and length of a pair, length of a KV head's line
-  static constexpr int kStart = start_tiles(kKind);
+  static constexpr int kStart = kStartTiles;
   __device__ __forceinline__ SequenceLine(const CachedAttnArgs& a, const Sequence& s) {
     n = blocks_of<kKind, D>(a, s);
     pairs = n / 2;
@@ -311,11 +311,11 @@ struct Segments {
     if (a.num_splits > 0 || a.parts[kKind].slots == 0 || blocks > kWholeRounds * a.parts[kKind].slots) return;
     const float work = a.c.heads_kv * wave_sum(lane_work);
     const int total = a.c.heads_kv * wave_sum(lane_line);
-    chunk = max((total + a.parts[kKind].slots - 1) / a.parts[kKind].slots, a.parts[kKind].min_tiles + start_tiles(kKind));
+    chunk = max((total + a.parts[kKind].slots - 1) / a.parts[kKind].slots, a.parts[kKind].min_tiles + kStartTiles);
     share = even_share<kKind, D>(a, batch, blocks, work, a.parts[kKind].slots);
     // (A chunk's workgroup starts one more segment than its length counts, and leaves two partials: the line has
     // to gain more than that.)
-    if (share > 0 && (!a.parts[kKind].line || share <= chunk + 2 * start_tiles(kKind))) {
+    if (share > 0 && (!a.parts[kKind].line || share <= chunk + 2 * kStartTiles)) {
       mode = kShares;
     } else if (kKind == kWide && a.parts[kKind].line) {
       mode = kLine;
@@ -369,7 +369,7 @@ struct Segments {
           const int at = position;
           leave<kKind>(a, item, -(Quotient(chunk).of(at + span.tiles - 1) - static_cast<int>(blockIdx.x) + 1));
         }
-        position = __builtin_amdgcn_readfirstlane(min(end, start + span.start + span.tiles + start_tiles(kKind)));
+        position = __builtin_amdgcn_readfirstlane(min(end, start + span.start + span.tiles + kStartTiles));
         if (any) return true;
         break;
       }

@@ -8,10 +8,11 @@
 //   o = sum_j softmax(s)_j v_j, lse = log sum_j e^(s_j); no such j: o = 0, lse = -inf.
 //
 // Lengths are known on the device only. Sequences with few rows (tokens x heads of a group) are bound by
-// reading the cache and run on cached_narrow.hip, those with many by the matrix cores and run on
-// cached_wide.hip; without cu_seqlens the host knows which it is, and only that kernel is launched.
-// Every workgroup of either derives the same list of items from the lengths (find_item, cached.hpp) and
-// takes the one of its own number; the grid is an upper bound from the sizes. Where the items are few, keys
+// reading the cache and run the narrow form (cached_narrow.hpp), those with many by the matrix cores and run the
+// wide one (cached_wide.hip). The host knows which there can be: calls with only few rows launch
+// cached_narrow.hip, calls without cu_seqlens and with many the wide kernel alone, and ragged batches the
+// wide kernel with both. Every workgroup derives the same schedule from the lengths (Segments, cached.hpp) and
+// takes its own part of it; the grid is an upper bound from the sizes. Where blocks of rows are few, their keys
 // are split over several workgroups, and a last kernel, here, merges the partials in order.
 #include "cached.hpp"
 
@@ -131,7 +132,7 @@ CachedPlan::Part plan_part(const CachedAttnArgs& args, Kind kind, int64_t least,
   } else if (args.num_splits == 0 && tiles > min_tiles && least <= kWholeRounds * resident && !whole) {
     part.slots = static_cast<int>(resident);
     // The line needs blocks enough, and positions that fit 32 bits.
-    part.line = kind == kWide && 4 * most > resident && most * (tiles + start_tiles(kind) + 1) < (int64_t{1} << 30);
+    part.line = kind == kWide && 4 * most > resident && most * (tiles + kStartTiles + 1) < (int64_t{1} << 30);
     const int64_t shares = most * ((tiles + min_tiles - 1) / min_tiles);
     part.partials = part.line ? 2 * resident : shares < resident ? shares : resident;
     part.workgroups = part.line || part.partials == resident ? resident : part.partials;

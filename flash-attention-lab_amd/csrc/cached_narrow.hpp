@@ -2,17 +2,19 @@
 // drafted tokens, short turns. Such a call is bound by reading the cache: 2 x (D + 1) bytes a key and KV head
 // in e4m3, against 4 D operations per row.
 //
-//  * A workgroup has one item, a key range of one KV head of one sequence. Its 4 waves take tiles of 32 keys
-//    of their own, w, w + 4, .., loaded into registers a tile early; no barriers until the waves' states
-//    are merged at the end.
+//  * A workgroup has one item, a key range of one KV head of one sequence. Its waves (4, or 8 where a CU holds
+//    one workgroup) take tiles of 32 keys of their own, w, w + waves, .., loaded into registers a tile early; no
+//    barriers until the waves' states are merged at the end.
 //  * Products are on v_mfma_f32_16x16x32, 16 rows to a column block (kCols blocks): with 16 rows or fewer
 //    (most decode steps) that is half the 32 x 32 form's work and registers, and four workgroups fit a CU
 //    instead of two. Scores are transposed, S^T = K Q^T: lane l holds row l % 16 and keys 4 (l / 16) .. + 3
 //    of each 16-key block, and the output O^T = V^T P^T, so softmax state and rescaling are per lane.
 //  * Every load instruction of a wave covers whole rows: reading half of each row's 128 bytes per instruction
-//    took 142 us for 8 sequences of 32K keys in e4m3, 173 with the streaming hint, whole rows FILL_WHOLE. So
-//    both tensors go through LDS to get to the lanes that multiply them, 8 KiB of the wave's own that holds
-//    K's tile, as it is in memory, and then V's (a wave's LDS operations keep their order).
+//    took 142 us for 8 sequences of 32K keys of 8 KV heads in e4m3, 173 with the streaming hint, whole rows 94-100
+//    (5.5-5.8 TB/s). So both tensors go through LDS to get to the lanes that multiply them, 8 KiB of the wave's
+//    own that holds K's tile, as it is in memory, and then V's (a wave's LDS operations keep their order).
+//  * Latency bounds short caches (1 sequence of 640 keys, 9.4 us on eight waves, 10.5 on four) and the start of
+//    all calls: 1.7 us for the schedule, 0.9 for the item, 1.8 to the first loads, 2.5 to their rows.
 //  * K's A operand: lane (m, g) = (l % 16, l / 16) takes 16 bytes of every 64 of key m's row. The products
 //    sum over dims in any order, and Q's fragments are read in the same one (step_dim).
 //  * V^T's operand needs keys across, so V goes into LDS in the tokens' type and comes back by
@@ -333,8 +335,7 @@ __device__ __forceinline__ void narrow_item(const CachedAttnArgs& a, const Item&
   }
 }
 
-// o = 0 and lse = -inf in the rows of the call that belong to no sequence. (A ragged call always launches
-// this kernel.)
+// o = 0 and lse = -inf in the rows of the call that belong to no sequence.
 template <int D>
 __device__ __forceinline__ void clear_unowned(const CachedAttnArgs& a) {
   if (a.c.cu_seqlens == nullptr) return;
