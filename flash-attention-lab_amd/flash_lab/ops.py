@@ -400,7 +400,8 @@ def attention_cached(
     shape without D. A token that sees no key gets o = 0 and lse = -inf, and so do rows of q behind the last
     sequence. Values of seq_lens, cu_seqlens and block_tables are not checked on the host (that would force
     a device sync): the kernels clamp them, so that a wrong one gives wrong rows and no access out of
-    bounds. A token's last bits can depend on the other sequences' lengths.
+    bounds. Keys and values that a token does not see do not reach it, whatever they hold. A token's last bits
+    can depend on the other sequences' lengths.
     """
     out, lse = _attention_cached(q, k_cache, v_cache, seq_lens, cu_seqlens, block_tables, k_scales, v_scales,
                                  causal, softmax_scale, impl, 0)
