@@ -311,6 +311,12 @@ struct Segments {
       return;
     }
     if (a.num_splits > 0 || a.parts[kKind].slots == 0 || blocks > kWholeRounds * a.parts[kKind].slots) return;
+    // (The grid is made for whole blocks too, which can be more; a workgroup that comes behind the slots starts
+    // when another has ended, and has nothing to do unless blocks stay whole.)
+    if (static_cast<int>(blockIdx.x) >= a.parts[kKind].slots && (a.parts[kKind].line || blocks <= a.parts[kKind].slots)) {
+      mode = kDone;
+      return;
+    }
     const float work = a.c.heads_kv * wave_sum(lane_work);
     const int total = a.c.heads_kv * wave_sum(lane_line);
     chunk = max((total + a.parts[kKind].slots - 1) / a.parts[kKind].slots, a.parts[kKind].min_tiles + kStartTiles);
@@ -321,8 +327,7 @@ struct Segments {
       mode = kShares;
     } else if (kKind == kWide && a.parts[kKind].line) {
       mode = kLine;
-      // (There can be more workgroups than slots; blockIdx.x chunk is below total + chunk for those that are not.)
-      position = static_cast<int>(blockIdx.x) < a.parts[kKind].slots ? min(static_cast<int>(blockIdx.x) * chunk, total) : total;
+      position = min(static_cast<int>(blockIdx.x) * chunk, total);  // (the product is below total + chunk and a few)
       end = min(position + chunk, total);
       position = __builtin_amdgcn_readfirstlane(position);
       end = __builtin_amdgcn_readfirstlane(end);
