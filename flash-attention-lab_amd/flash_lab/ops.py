@@ -401,7 +401,8 @@ def attention_cached(
     sequence. Values of seq_lens, cu_seqlens and block_tables are not checked on the host (that would force
     a device sync): the kernels clamp them, so that a wrong one gives wrong rows and no access out of
     bounds. Keys and values that a token does not see do not reach it, whatever they hold. A token's last bits
-    can depend on the other sequences' lengths.
+    can depend on the other sequences' lengths. A batch with one token for every sequence is faster as [B, 1, H, D]
+    without cu_seqlens, or through decode: then no longer sequences are prepared for.
     """
     out, lse = _attention_cached(q, k_cache, v_cache, seq_lens, cu_seqlens, block_tables, k_scales, v_scales,
                                  causal, softmax_scale, impl, 0)
