@@ -21,8 +21,11 @@ constexpr int kKeys = 64;        // keys of a tile: splits are whole tiles
 // 1,914 tokens, bf16 268-274 / 245-253 / 242-247; 24, 32/32 heads of 64, 5,975 tokens, bf16 394-401 / 376-382 / 379-381;
 // 8, 16/16 heads of 64, 2,377 tokens, e4m3 102 / 97 / 100.
 constexpr int kStartTiles = 6;
-// From so many rounds of blocks on they run whole, as they come, the longest first.
-constexpr int kWholeRounds = 6;
+// From so many rounds of blocks on they run whole, as they come, the longest first: what the line evens out no
+// longer pays for its partials. us with the merge, whole / line, bf16 if not said: 3.1 rounds (16 sequences, 64/8 heads
+// of 128, 3,135 tokens on up to 8,000, e4m3) 663-681 / 685; 3.2 (12, 32/32 heads of 64, up to 700 tokens on 2,200)
+// 103 / 108; 3.5 (16, 32/8 of 128) 180 / 184; 4.3 (24, 32/32 of 64, on up to 8,000) 355-360 / 361-381; 12.5 406-420 / 403.
+constexpr int kWholeRounds = 3;
 // Rows of a block.
 __host__ __device__ __forceinline__ constexpr int block_rows(Kind kind) { return kind == kNarrow ? kNarrowRows : 256; }
 
